@@ -47,8 +47,9 @@ typedef enum rb_status {
     RB_SERVER_UNHEALTHY = 8  /* ServerError::ServerUnhealthy{errors}, runtime/mod.rs:645-661    */
 } rb_status;
 
-/* ruda_core::tensor::DType values used on this path (runtime/hccl.rs:97-111 lists the same set). */
-typedef enum rb_dtype { RB_F32 = 0, RB_F16 = 1, RB_BF16 = 2, RB_I32 = 3, RB_I64 = 4, RB_U8 = 5 } rb_dtype;
+/* ruda_core::tensor::DType values used on this path (runtime/hccl.rs:97-111 lists the same set), and RB_I8 for rows held in
+ * 8 bits (rb_quantize_rows, rb_rms_norm_quant, rb_linear_i8), which the reference does not have. */
+typedef enum rb_dtype { RB_F32 = 0, RB_F16 = 1, RB_BF16 = 2, RB_I32 = 3, RB_I64 = 4, RB_U8 = 5, RB_I8 = 6 } rb_dtype;
 
 /* Transpose, rust-ascend-driver/src/tensor/deepgemm/plan.rs. */
 typedef enum rb_transpose { RB_NO_TRANSPOSE = 0, RB_TRANSPOSE = 1 } rb_transpose;
@@ -321,6 +322,58 @@ RB_API int32_t rb_linear_host(rb_ctx* ctx, const void* host_x, const rb_tensor* 
  * that reason it returns RB_INVALID_TENSOR between rb_graph_begin and rb_graph_end. */
 RB_API int32_t rb_gemm_no_alloc(rb_ctx* ctx, const rb_tensor* a, const rb_tensor* b, int32_t transpose_a, int32_t transpose_b,
                                 const rb_tensor* out);
+
+/* ---- rows held in 8 bits, and the linear on them ------------------------------------------------------------------- */
+/* Rules shared by the entries of this section.  A row of values y is held as signed 8-bit integers q and one FP32 scale:
+ * scale = max(max|y| / 127, 2^-126), q = y / scale rounded to the nearest integer (ties to even), so |q| <= 127 and
+ * |q * scale - y| <= scale / 2.  A row that holds a NaN or an infinity gets a NaN scale and zeros, so that everything computed from
+ * it is NaN.  Row-strided inputs: the last axis is contiguous and the leading axes step through rows at one distance (a column
+ * range of a wider tensor); only the element's own alignment is required of them. */
+/* This entry has no counterpart in the reference.  rb_rms_norm (delta NULL, x_out NULL) or rb_add_rms_norm (both given: the sum
+ * is rounded to x's type and stored to x_out, which may be x itself) whose result leaves in 8 bits: y = s * rsqrt(mean(s^2) +
+ * epsilon) * w is quantised by rows into q (I8, x's shape) and scales (FP32, one value per row).  x F32, BF16 or F16, any width;
+ * weight in x's type or F32.  One pass over x: the normalised row is never stored. */
+RB_API int32_t rb_rms_norm_quant(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* delta, const rb_tensor* weight, double epsilon,
+                                 const rb_tensor* x_out, const rb_tensor* q, const rb_tensor* scales);
+/* This entry has no counterpart in the reference.  Quantises rows: y = x, or, with `up` given, y = SiLU(x) * up in FP32 (the
+ * feed-forward's rb_silu_mul with its result in 8 bits).  x and up: equal shape and type (F32, BF16 or F16), row-strided, so gate
+ * and up may be the two halves of one projection's output; q I8 contiguous of that shape, scales FP32 with one value per row.
+ * Weights [N, K] quantised this way have the scale per output channel that rb_linear_i8 takes. */
+RB_API int32_t rb_quantize_rows(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* up, const rb_tensor* q, const rb_tensor* scales);
+/* This entry has no counterpart in the reference.  y = q * scale of its row, one FP32 product rounded to y's type (F32, BF16 or
+ * F16). */
+RB_API int32_t rb_dequantize_rows(rb_ctx* ctx, const rb_tensor* q, const rb_tensor* scales, const rb_tensor* y);
+/* This entry has no counterpart in the reference (its fixed-weight linear, runtime/mod.rs:383-385, holds BF16).  Linear on 8-bit
+ * integers: y[m, n] = (sum over k of x[m, k] w[n, k]) * (x_scales[m] * w_scales[n]) (+ bias[n]).  x I8 [.., K], w I8 [N, K], x_scales
+ * FP32 with one value per row of x, w_scales FP32 [N], bias FP32 [N] or NULL, y F32, BF16 or F16 [.., N].  The integer sum is exact
+ * (32-bit), so the result does not depend on how the work is split; it is rounded to FP32 once, scaled, biased and rounded to
+ * y's type.  Any number of rows, any N; K a multiple of 16 within 131056 (the largest whose sum cannot leave 32 bits). */
+RB_API int32_t rb_linear_i8(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* x_scales, const rb_tensor* w, const rb_tensor* w_scales,
+                            const rb_tensor* bias, const rb_tensor* y);
+
+/* ---- scores of single tokens ------------------------------------------------------------------------------------------ */
+#define RB_MAX_TOP 64
+/* This entry has no counterpart in the reference (its loss, src/nn/causal_lm.rs:118-196, keeps only the sum).  With z = scale *
+ * logits (scale > 0: one over the temperature) and lse = log(sum(exp(z))), for every row: log_probs = z[id] - lse, lse, entropy =
+ * lse - sum(softmax(z) z), and the top_k largest entries with their log probabilities, ordered by logit (largest first, equal
+ * logits by lowest index; a NaN counts as the largest).  logits F32, BF16 or F16 [.., V], row-strided; ids I32 or I64 with one
+ * value per row; log_probs, lse and entropy (the last nullable) FP32 with one value per row; top_values FP32 and top_ids I32
+ * [rows, top_k], 0 <= top_k <= RB_MAX_TOP and <= V, both NULL when top_k is 0.  A row whose id is ignore_index has log_probs 0;
+ * its other outputs are those of its logits.  An id outside [0, V) is never used as an index: its row counts as ignored, and a
+ * synchronous context returns RB_INVALID_TENSOR for the call.  Logits of -inf have probability 0;
+ * a row without any finite logit (its lse is -inf), or with a NaN or +inf, gives NaN. */
+RB_API int32_t rb_token_log_probs(rb_ctx* ctx, const rb_tensor* logits, const rb_tensor* ids, float scale, int64_t ignore_index,
+                                  const rb_tensor* log_probs, const rb_tensor* lse, const rb_tensor* entropy, uint32_t top_k,
+                                  const rb_tensor* top_values, const rb_tensor* top_ids);
+/* This entry has no counterpart in the reference.  Gradient of rb_token_log_probs with respect to the logits, from the saved lse
+ * and entropy: dlogits[v] = scale * (g (onehot(id)[v] - p[v]) - h p[v] (log p[v] + entropy)), p = exp(z - lse), g = grad_log_probs of
+ * the row (0 for ignored rows), h = grad_entropy (NULL: 0; entropy may then be NULL too).  A row with g = h = 0 gets zeros whatever
+ * its logits hold.  p inherits the rounding of lse (|lse| 2^-24, relative); an lse of 2^22 or more in magnitude (a row of nothing but
+ * a mask's lowest value) no longer tells the logits apart and gives a NaN row.  dlogits has the type and shape of the logits, may be row-strided, and may be the logits tensor itself; columns
+ * between its rows keep their bits. */
+RB_API int32_t rb_token_log_probs_backward(rb_ctx* ctx, const rb_tensor* logits, const rb_tensor* ids, float scale, int64_t ignore_index,
+                                           const rb_tensor* lse, const rb_tensor* entropy, const rb_tensor* grad_log_probs,
+                                           const rb_tensor* grad_entropy, const rb_tensor* dlogits);
 
 /* ---- attention --------------------------------------------------------------------------------------- */
 /* nn::scaled_dot_product_attention_bf16_fp32 / causal_attention / grouped_query_attention /

@@ -70,6 +70,24 @@ bool same_shape(const rb_tensor* a, const rb_tensor* b);
 // Rows and width of a last-axis operation.
 void rows_width(const rb_tensor* t, uint64_t* rows, uint64_t* width);
 
+// Address and rows of a row-strided tensor: the last axis is contiguous and the leading axes collapse into `rows` rows that start
+// `ld` elements apart.  Only the element's own alignment is required; the byte range that the strides reach must lie inside the
+// storage.  `extent_bytes` is the length of that range.
+struct Rows { void* ptr = nullptr; uint64_t rows = 0, width = 0, ld = 0, extent_bytes = 0; };
+int32_t resolve_rows(rb_ctx* ctx, const rb_tensor* t, const char* what, Rows* out);
+
+// Makes the context's device current for the length of a call and puts the caller's back.
+struct DeviceGuard {
+    int before = -1;
+    explicit DeviceGuard(const rb_ctx* ctx) {
+        int now = -1;
+        if (cudaGetDevice(&now) == cudaSuccess && now != ctx->device && cudaSetDevice(ctx->device) == cudaSuccess) before = now;
+    }
+    ~DeviceGuard() { if (before >= 0) cudaSetDevice(before); }
+    DeviceGuard(const DeviceGuard&) = delete;
+    DeviceGuard& operator=(const DeviceGuard&) = delete;
+};
+
 // Called after every kernel launch: records launch failures on the sticky list, counts the launch
 // and synchronises when the context runs in the reference's synchronous mode.
 int32_t after_launch(rb_ctx* ctx, const char* operation);

@@ -18,14 +18,14 @@ size_t dtype_size(uint32_t dtype) {
         case RB_F32: case RB_I32: return 4;
         case RB_F16: case RB_BF16: return 2;
         case RB_I64: return 8;
-        case RB_U8: return 1;
+        case RB_U8: case RB_I8: return 1;
         default: return 0;
     }
 }
 const char* dtype_name(uint32_t dtype) {
     switch (dtype) {
         case RB_F32: return "F32"; case RB_F16: return "F16"; case RB_BF16: return "BF16";
-        case RB_I32: return "I32"; case RB_I64: return "I64"; case RB_U8: return "U8";
+        case RB_I32: return "I32"; case RB_I64: return "I64"; case RB_U8: return "U8"; case RB_I8: return "I8";
         default: return "unknown";
     }
 }
@@ -82,6 +82,49 @@ int32_t resolve(rb_ctx* ctx, const rb_tensor* t, const char* what, void** out, b
     char* p = (char*)s.ptr + t->offset;
     if (((uintptr_t)p & 15u) != 0) return fail(RB_INVALID_TENSOR, "%s: device address must be 16-byte aligned", what);
     *out = p;
+    return RB_OK;
+}
+
+int32_t resolve_rows(rb_ctx* ctx, const rb_tensor* t, const char* what, Rows* out) {
+    *out = Rows{};
+    if (!t) return fail(RB_INVALID_TENSOR, "%s: missing tensor", what);
+    if (t->rank == 0 || t->rank > 8) return fail(RB_INVALID_TENSOR, "%s: rank must be within 1..8", what);
+    const size_t es = dtype_size(t->dtype);
+    if (!es) return fail(RB_INVALID_TENSOR, "%s: unsupported dtype %u", what, t->dtype);
+    const uint64_t width = t->shape[t->rank - 1];
+    if (width > 1 && t->strides[t->rank - 1] != 1) return fail(RB_INVALID_TENSOR, "%s: the last axis must be contiguous", what);
+    // Axes of extent one carry no stride; each remaining leading axis has to continue the one inside it.
+    const uint64_t limit = uint64_t(1) << 62;
+    uint64_t rows = 1, ld = 0;
+    bool known = false, empty = width == 0;
+    for (uint32_t i = 0; i + 1 < t->rank; ++i) empty = empty || t->shape[i] == 0;
+    for (int i = (int)t->rank - 2; i >= 0 && !empty; --i) {
+        const uint64_t extent = t->shape[i];
+        if (extent == 1) continue;
+        if (t->strides[i] > limit || extent > limit / rows) return fail(RB_INVALID_TENSOR, "%s: strides reach outside the storage", what);
+        if (!known) { ld = t->strides[i]; known = true; }
+        else if (ld > limit / rows || t->strides[i] != ld * rows) return fail(RB_INVALID_TENSOR, "%s: the leading axes must step through rows at one distance", what);
+        rows *= extent;
+    }
+    if (empty) { uint64_t w; rows_width(t, &rows, &w); }
+    if (!known) ld = width;
+    Storage s;
+    {
+        std::lock_guard<std::mutex> g(ctx->lock);
+        auto it = ctx->storage.find(t->handle);
+        if (it == ctx->storage.end()) return fail(RB_NULL_HANDLE, "%s: unknown storage handle %llu", what, (unsigned long long)t->handle);
+        s = it->second;
+    }
+    if (t->offset > s.bytes) return fail(RB_INVALID_TENSOR, "%s: strides reach outside the storage", what);
+    uint64_t bytes = 0;
+    if (!empty) {
+        const uint64_t room = (s.bytes - t->offset) / es;
+        if (width > room || (rows > 1 && ld > (room - width) / (rows - 1))) return fail(RB_INVALID_TENSOR, "%s: strides reach outside the storage", what);
+        bytes = ((rows - 1) * ld + width) * es;
+    }
+    char* p = (char*)s.ptr + t->offset;
+    if (((uintptr_t)p) % es) return fail(RB_INVALID_TENSOR, "%s: device address must be aligned to its element", what);
+    out->ptr = p; out->rows = rows; out->width = width; out->ld = ld; out->extent_bytes = bytes;
     return RB_OK;
 }
 

@@ -26,15 +26,16 @@ class DType(enum.IntEnum):
     I32 = 3
     I64 = 4
     U8 = 5
+    I8 = 6
 
     @property
     def size(self) -> int:
-        return {0: 4, 1: 2, 2: 2, 3: 4, 4: 8, 5: 1}[int(self)]
+        return {0: 4, 1: 2, 2: 2, 3: 4, 4: 8, 5: 1, 6: 1}[int(self)]
 
     @property
     def numpy(self):
         """Host carrier type: BF16 travels as its 16-bit pattern."""
-        return {0: np.float32, 1: np.float16, 2: np.uint16, 3: np.int32, 4: np.int64, 5: np.uint8}[int(self)]
+        return {0: np.float32, 1: np.float16, 2: np.uint16, 3: np.int32, 4: np.int64, 5: np.uint8, 6: np.int8}[int(self)]
 
 
 class Transpose(enum.IntEnum):
@@ -126,9 +127,16 @@ class TensorBuffer:
 
     def __post_init__(self):
         self.shape = tuple(int(d) for d in self.shape)
-        if self.strides is None:
-            self.strides = _contiguous_strides(self.shape)
+        self.strides = _contiguous_strides(self.shape) if self.strides is None else tuple(int(d) for d in self.strides)
         self.dtype = DType(self.dtype)
+
+    def __setattr__(self, name, value):
+        # The C descriptor is made on first use and describes the fields as they are: a changed field drops it.
+        object.__setattr__(self, name, value)
+        self.__dict__.pop("_descriptor", None)
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_descriptor"}
 
     @property
     def elements(self) -> int:
@@ -153,15 +161,16 @@ class TensorBuffer:
     def _c(self) -> rb_tensor:
         if not 1 <= len(self.shape) <= 8:
             raise InvalidTensor("tensor rank must be within 1..8")
-        t = rb_tensor()
-        t.handle, t.offset, t.dtype, t.rank = self.handle, self.offset, int(self.dtype), len(self.shape)
-        for i, (d, s) in enumerate(zip(self.shape, self.strides)):
-            t.shape[i], t.strides[i] = d, s
-        return t
+        return rb_tensor(self.handle, self.offset, int(self.dtype), len(self.shape), tuple(self.shape), tuple(self.strides))
 
 
 def _ref(t: TensorBuffer | None):
-    return None if t is None else C.byref(t._c())
+    if t is None:
+        return None
+    d = t.__dict__.get("_descriptor")
+    if d is None:
+        d = t.__dict__["_descriptor"] = C.byref(t._c())
+    return d
 
 
 class ComputeClient:
@@ -228,7 +237,8 @@ class ComputeClient:
         arr = np.ascontiguousarray(array)
         if dtype is None:
             dtype = {np.dtype(np.float32): DType.F32, np.dtype(np.float16): DType.F16, np.dtype(np.uint16): DType.BF16,
-                     np.dtype(np.int32): DType.I32, np.dtype(np.int64): DType.I64, np.dtype(np.uint8): DType.U8}[arr.dtype]
+                     np.dtype(np.int32): DType.I32, np.dtype(np.int64): DType.I64, np.dtype(np.uint8): DType.U8,
+                     np.dtype(np.int8): DType.I8}[arr.dtype]
         if arr.dtype != np.dtype(DType(dtype).numpy):
             raise InvalidTensor(f"host array dtype {arr.dtype} does not carry {DType(dtype).name}")
         return self._owned(self.create_from_slice(arr), arr.shape if arr.ndim else (1,), dtype)
@@ -349,6 +359,14 @@ class B200Runtime:
             n *= d
         return n
 
+    @staticmethod
+    def _outputs(out, count: int) -> list:
+        """The caller's result tensors, padded with None; more than the operator has is an error."""
+        out = list(out) if out is not None else []
+        if len(out) > count:
+            raise InvalidTensor(f"at most {count} output tensors are taken")
+        return out + [None] * (count - len(out))
+
     # -- row programs ----------------------------------------------------------------------------
     @staticmethod
     def rms_norm(client: ComputeClient, input: TensorBuffer, weight: TensorBuffer, epsilon: float, out_dtype: DType | None = None):
@@ -366,6 +384,76 @@ class B200Runtime:
         mean, rstd = client.tensor((rows,), DType.F32), client.tensor((rows,), DType.F32)
         _check(client._lib.rb_layer_norm(client._ctx, _ref(input), _ref(weight), _ref(bias), C.c_double(epsilon), _ref(out), _ref(mean), _ref(rstd)))
         return [out, mean, rstd]
+
+    # -- rows held in 8 bits (no counterpart in the reference) ---------------------------------------------------------
+    @staticmethod
+    def rms_norm_quant(client: ComputeClient, input: TensorBuffer, weight: TensorBuffer, epsilon: float, delta: TensorBuffer | None = None, out=None):
+        """RMSNorm of `input`, or of `input + delta` rounded to the input's type, with its result as I8 rows: rb_rms_norm_quant.
+        Returns [q, scales], and the sum as a third entry where `delta` is given.  `out` = (q, scales[, sum]) writes into the
+        caller's tensors instead of new ones (the sum may be `input` itself)."""
+        q, scales, total = B200Runtime._outputs(out, 3)
+        q = q or client.tensor(input.shape, DType.I8)
+        scales = scales or client.tensor(input.shape[:-1] or (1,), DType.F32)
+        if delta is not None and total is None:
+            total = client.tensor(input.shape, input.dtype)
+        _check(client._lib.rb_rms_norm_quant(client._ctx, _ref(input), _ref(delta), _ref(weight), C.c_double(epsilon), _ref(total), _ref(q), _ref(scales)))
+        return [q, scales] + ([total] if delta is not None else [])
+
+    @staticmethod
+    def quantize_rows(client: ComputeClient, input: TensorBuffer, up: TensorBuffer | None = None, out=None):
+        """[q, scales]: rows of `input`, or of SiLU(input) * up, as I8 with one FP32 scale a row (rb_quantize_rows).  Both inputs may be
+        column ranges of wider tensors.  `out` = (q, scales) writes into the caller's tensors."""
+        q, scales = B200Runtime._outputs(out, 2)
+        q = q or client.tensor(input.shape, DType.I8)
+        scales = scales or client.tensor(input.shape[:-1] or (1,), DType.F32)
+        _check(client._lib.rb_quantize_rows(client._ctx, _ref(input), _ref(up), _ref(q), _ref(scales)))
+        return [q, scales]
+
+    @staticmethod
+    def dequantize_rows(client: ComputeClient, q: TensorBuffer, scales: TensorBuffer, dtype: DType = DType.BF16, out: TensorBuffer | None = None) -> TensorBuffer:
+        """q * scale of its row, in `dtype` or in the type of `out` (rb_dequantize_rows)."""
+        out = out or client.tensor(q.shape, dtype)
+        _check(client._lib.rb_dequantize_rows(client._ctx, _ref(q), _ref(scales), _ref(out)))
+        return out
+
+    @staticmethod
+    def linear_i8(client: ComputeClient, input: TensorBuffer, input_scales: TensorBuffer, weight: TensorBuffer, weight_scales: TensorBuffer,
+                  bias: TensorBuffer | None = None, dtype: DType = DType.BF16, out: TensorBuffer | None = None) -> TensorBuffer:
+        """Y = (X W^T) * (input_scales x weight_scales) (+ bias) for I8 X [.., K] and W [N, K] with one FP32 scale per row of each
+        (rb_linear_i8); exact integer sums, result in `dtype` or in the type of `out`."""
+        if len(weight.shape) != 2 or not input.shape:
+            raise InvalidTensor("8-bit linear takes X[..,K] and W[N,K]")
+        out = out or client.tensor(input.shape[:-1] + (weight.shape[0],), dtype)
+        _check(client._lib.rb_linear_i8(client._ctx, _ref(input), _ref(input_scales), _ref(weight), _ref(weight_scales), _ref(bias), _ref(out)))
+        return out
+
+    # -- scores of single tokens (no counterpart in the reference) -----------------------------------------------------
+    @staticmethod
+    def token_log_probs(client: ComputeClient, logits: TensorBuffer, ids: TensorBuffer, scale: float = 1.0, ignore_index: int = -100, top_k: int = 0, out=None):
+        """[log_probs, lse, entropy, top_values, top_ids] of rows of logits [.., V] scaled by `scale` (one over the temperature):
+        rb_token_log_probs.  The last two are None when top_k is 0.  `out` takes the five tensors in that order; entropy may be
+        None there to leave it out."""
+        rows = logits.shape[:-1] or (1,)
+        if out is None:
+            out = [client.tensor(rows, DType.F32) for _ in range(3)]
+            out += [client.tensor(rows + (top_k,), DType.F32), client.tensor(rows + (top_k,), DType.I32)] if top_k else [None, None]
+        log_probs, lse, entropy, top_values, top_ids = B200Runtime._outputs(out, 5)
+        if not 0 <= top_k <= 64:
+            raise InvalidTensor("top_k must be within 0..64 and the vocabulary")
+        _check(client._lib.rb_token_log_probs(client._ctx, _ref(logits), _ref(ids), C.c_float(scale), C.c_int64(ignore_index), _ref(log_probs), _ref(lse),
+                                              _ref(entropy), C.c_uint32(top_k), _ref(top_values), _ref(top_ids)))
+        return [log_probs, lse, entropy, top_values, top_ids]
+
+    @staticmethod
+    def token_log_probs_backward(client: ComputeClient, logits: TensorBuffer, ids: TensorBuffer, lse: TensorBuffer, entropy: TensorBuffer | None,
+                                 grad_log_probs: TensorBuffer, grad_entropy: TensorBuffer | None = None, scale: float = 1.0, ignore_index: int = -100,
+                                 out: TensorBuffer | None = None) -> TensorBuffer:
+        """Gradient of token_log_probs with respect to the logits from the saved lse and entropy (rb_token_log_probs_backward); `out`
+        may be `logits` itself."""
+        out = out or client.tensor(logits.shape, logits.dtype)
+        _check(client._lib.rb_token_log_probs_backward(client._ctx, _ref(logits), _ref(ids), C.c_float(scale), C.c_int64(ignore_index), _ref(lse),
+                                                       _ref(entropy), _ref(grad_log_probs), _ref(grad_entropy), _ref(out)))
+        return out
 
     @staticmethod
     def softmax(client: ComputeClient, input: TensorBuffer) -> TensorBuffer:

@@ -1,0 +1,217 @@
+"""GPU: log probabilities of given tokens, entropy, top alternatives and their gradient against the definitions in 64 bits.
+
+Tolerance of ln S.  A term 2^d is off by 2^-22 (the exponential) and by ln2 |d| 3 x 2^-24 (d's roundings); weighted with its share of the
+sum, the |d| are at most about log2 of the vocabulary (17).  A thread adds at most V / 256 + 16 terms one after the other (one rounding
+each), then 8 + 3 levels.  So |ln S| is off by D = 2^-22 + 17 ln2 3 x 2^-24 + (V / 256 + 27) x 2^-24 at most, T / S by that times 18 more.
+A log probability adds the roundings of scale (x - M) (three, relative); lse that of its result."""
+import numpy as np
+import pytest
+
+import eight_bit_reference as R
+from rust_ascend_b200 import B200Runtime as RT
+from rust_ascend_b200 import DType, TensorBuffer
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16, I32 = DType.F32, DType.F16, DType.BF16, DType.I32
+U = 2.0 ** -24
+
+
+def spread(vocab):
+    return 2.0 ** -22 + 17 * 0.7 * 3 * U + (vocab / 256 + 27) * U
+
+
+def compare(got, want, vocab, top):
+    log_prob, lse, entropy, values, ids = got
+    w_log_prob, w_lse, w_entropy, w_values, w_ids, _ = want
+    d = spread(vocab)
+    with np.errstate(invalid="ignore"):
+        for a, w, extra in ((log_prob, w_log_prob, 0), (lse, w_lse, 0), (entropy, w_entropy, 20 * d)) + (((values, w_values, 0),) if top else ()):
+            same = (np.isnan(a) & np.isnan(w)) | (a == w)
+            off = np.where(same, 0, np.abs(a - w) - (d + extra + 6 * U * np.abs(w)))
+            assert off.max(initial=0) <= 0, off.max()
+    if top:
+        assert np.array_equal(ids, w_ids)
+
+
+def call(client, x, xv, ids, dtype, scale, top, ignore=-100, view=None):
+    t = view if view is not None else client.upload(x, dtype)
+    out = RT.token_log_probs(client, t, client.upload(ids), scale=scale, ignore_index=ignore, top_k=top)
+    compare([None if o is None else client.read(o) for o in out], R.scores(xv, ids, scale, ignore, top), xv.shape[1], top)
+    return t, out
+
+
+def case(rows, vocab, dtype, seed=0, spread_of=2.5):
+    rng = np.random.default_rng([rows, vocab, seed])
+    x, xv = R.hold(rng.standard_normal((rows, vocab)) * spread_of, dtype)
+    ids = rng.integers(0, vocab, rows)
+    ids[rng.random(rows) < 0.2] = -100
+    return rng, x, xv, ids
+
+
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (3, 2, 2), (2, 7, 3), (5, 64, 64), (4, 257, 20), (7, 1000, 1), (3, 8192, 64), (1, 32000, 20), (2, 50001, 64), (1, 128000, 33),
+                                            (9, 4099, 5), (300, 3001, 7), (700, 515, 0), (40, 20011, 10)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_scores(client, rows, vocab, top, dtype):
+    rng, x, xv, ids = case(rows, vocab, dtype)
+    call(client, x, xv, ids, dtype, 1.25, top)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("pad,offset", [(1, 0), (64, 0), (5, 3)])
+def test_padded_rows_and_unaligned_starts(client, dtype, pad, offset):
+    rng, x, xv, ids = case(6, 5000 + pad, dtype)
+    x[:, :offset] = x[:, 5000 + offset:] = np.array(60000.0 if dtype != BF16 else 0x477f).astype(x.dtype)      # a large value: reading it would show
+    t = client.upload(x, dtype)
+    view = TensorBuffer(t.handle, (6, 5000 - offset), dtype, (5000 + pad, 1), offset * dtype.size, t._owner)
+    call(client, None, xv[:, offset:5000], np.where(ids >= 5000 - offset, 0, ids), dtype, 1.0, 8, view=view)
+
+
+@pytest.mark.parametrize("vocab", [100, 5000, 40000])
+@pytest.mark.parametrize("top", [0, 20, 64])
+def test_masked_and_special_rows(client, vocab, top):
+    """Masks by -inf and by the type's lowest value, rows without any logit, NaN, +inf, constant rows, both zeros, a single survivor."""
+    rng = np.random.default_rng(vocab + top)
+    x = (rng.standard_normal((12, vocab)) * 2).astype(np.float32)
+    keep = rng.integers(0, vocab, 5)
+    for r, masked in ((0, -np.inf), (1, np.finfo(np.float32).min)):
+        row = np.full(vocab, masked, np.float32)
+        row[keep] = x[r, keep]
+        x[r] = row
+    x[2] = -np.inf
+    x[3, vocab // 3] = np.nan
+    x[4, vocab // 2] = np.inf
+    x[5] = 1.5
+    x[6] = 0.0
+    x[6, ::3] = -0.0
+    x[7] = -np.inf
+    x[7, vocab - 1] = -4.0
+    x[8] = np.arange(vocab)[::-1] * 1e-3
+    x[9] = np.arange(vocab) * 1e-3
+    x[10] = np.round(x[10])                           # many ties everywhere
+    x[11] = np.finfo(np.float32).min
+    ids = rng.integers(0, vocab, 12)
+    ids[0], ids[7] = keep[0], vocab - 1
+    ids[11] = -100
+    call(client, x, x, ids, F32, 0.7, top)
+
+
+def test_hostile_order_for_the_top_list(client):
+    """The largest values sit in few slices of every split, far more of them than are asked for."""
+    vocab = 60000
+    x = np.random.default_rng(0).standard_normal((4, vocab)).astype(np.float32)
+    for r, period in enumerate((256 * 4, 2048, 8, 512)):
+        at = np.arange(vocab) % period < 8
+        x[r, at] += 100
+    ids = np.zeros(4, np.int64)
+    call(client, x, x, ids, F32, 1.0, 64)
+    x, xv = R.hold(x, BF16)
+    call(client, x, xv, ids, BF16, 1.0, 17)
+
+
+def test_ids_outside_the_vocabulary_and_other_ignore_index(client):
+    rng, x, xv, ids = case(8, 300, F32)
+    ids[:4] = (300, -1, 2**40, 7)
+    call(client, x, xv, ids, F32, 1.0, 2, ignore=7)
+    call(client, x, xv, np.where(np.abs(ids) > 2**31 - 1, 300, ids).astype(np.int32), F32, 1.0, 2, ignore=7)
+
+
+def test_outputs_may_be_left_out_and_neighbours_stay(client):
+    rng, x, xv, ids = case(5, 777, F32)
+    t, i = client.upload(x), client.upload(ids)
+    full = RT.token_log_probs(client, t, i)
+    out = [client.tensor((5,), F32), client.tensor((5,), F32), None]
+    RT.token_log_probs(client, t, i, out=out)
+    for a, b in zip(full[:2], out):
+        assert np.array_equal(client.read(a), client.read(b))
+
+
+# ---- gradient --------------------------------------------------------------------------------------------------------------------
+def gradient_error(xv, ids, scale, g, h, dtype):
+    """How far an element may be off: p by the exponential, z - lse and the saved lse, the bracket by its roundings, the result by its storage."""
+    _, lse, entropy, _, _, live = R.scores(xv, ids, scale, -100, 0)
+    z = xv.astype(np.float64) * scale
+    lp = z - lse[:, None]
+    p = np.exp(lp)
+    d = spread(xv.shape[1])
+    bracket = np.abs(np.where(live, g, 0))[:, None] + np.abs(h)[:, None] * (np.abs(np.where(p > 0, lp, 0)) + np.abs(entropy)[:, None])
+    rel = 2.0 ** -21 + 4 * U * (np.abs(np.where(p > 0, z, 0)) + np.abs(lse)[:, None]) + d
+    return scale * (p * bracket * (rel + 8 * U) + p * np.abs(h)[:, None] * (22 * d) + 4 * U * np.abs(np.where(live, g, 0))[:, None] * p) + 2.0 ** -140
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (2, 5), (7, 1000), (33, 4097), (5, 20011), (2, 128000), (600, 300)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("with_entropy", [False, True])
+def test_gradient(client, rows, vocab, dtype, with_entropy):
+    rng, x, xv, ids = case(rows, vocab, dtype)
+    g, h = rng.standard_normal(rows).astype(np.float32), (rng.standard_normal(rows) * 0.3).astype(np.float32) * with_entropy
+    t, out = call(client, x, xv, ids, dtype, 1.25, 0)
+    up = client.upload
+    d = RT.token_log_probs_backward(client, t, up(ids), out[1], out[2] if with_entropy else None, up(g), up(h) if with_entropy else None, scale=1.25)
+    got, want = R.read(client, d), R.scores_gradient(xv, ids, 1.25, -100, g, h)
+    half = R.half_step(dtype)
+    smallest = {F32: 2.0 ** -149, BF16: 2.0 ** -133, F16: 2.0 ** -24}[dtype]
+    off = np.abs(got - want) - (gradient_error(xv, ids, 1.25, g, h, dtype) * (1 + half) + (half + 6 * U) * np.abs(want) + smallest)
+    assert off.max() <= 0, off.max()
+    # in place, and with rows of another alignment
+    copy = up(x, dtype)
+    RT.token_log_probs_backward(client, copy, up(ids), out[1], out[2], up(g), up(h), scale=1.25, out=copy)
+    again = RT.token_log_probs_backward(client, t, up(ids), out[1], out[2], up(g), up(h), scale=1.25)
+    assert np.array_equal(R.read(client, copy), R.read(client, again))
+    wide = up(np.zeros((rows, vocab + 3), x.dtype), dtype)
+    view = TensorBuffer(wide.handle, (rows, vocab), dtype, (vocab + 3, 1), dtype.size, wide._owner)
+    RT.token_log_probs_backward(client, t, up(ids), out[1], out[2], up(g), up(h), scale=1.25, out=view)
+    held = R.read(client, wide)
+    assert np.array_equal(held[:, 1:vocab + 1], R.read(client, again)) and not held[:, 0].any() and not held[:, vocab + 1:].any()
+
+
+def test_gradient_against_differences(client):
+    """Central differences of the 64-bit scores along random directions.  A difference over 2e-4 leaves an error of its square (the third
+    derivative is of order one) times the direction's norm; the gradient's own FP32 error is below 1e-5 of the same norm."""
+    rng, x, xv, ids = case(4, 500, F32, seed=5)
+    g, h = rng.standard_normal(4).astype(np.float32), rng.standard_normal(4).astype(np.float32)
+    t, out = call(client, x, xv, ids, F32, 0.8, 0)
+    d = client.read(RT.token_log_probs_backward(client, t, client.upload(ids), out[1], out[2], client.upload(g), client.upload(h), scale=0.8)).astype(np.float64)
+
+    def loss(v):
+        chosen, _, entropy, _, _, _ = R.scores(v, ids, 0.8, -100, 0)
+        return (g * chosen + h * entropy).sum()
+    for _ in range(6):
+        u = rng.standard_normal(x.shape)
+        step = 2e-4
+        want = (loss(x + step * u) - loss(x - step * u)) / (2 * step)
+        assert abs((d * u).sum() - want) <= 1e-5 * np.linalg.norm(u) + 1e-6
+
+
+def test_gradient_of_masked_and_idle_rows(client):
+    vocab = 3000
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((6, vocab)).astype(np.float32)
+    x[0, 10:] = -np.inf
+    x[1, ::2] = np.finfo(np.float32).min
+    x[2] = np.nan                                     # ignored and without upstream: padding may hold anything
+    x[3] = -np.inf                                    # scored: NaN
+    x[5] = np.nan
+    x = np.concatenate([x, np.full((1, vocab), np.finfo(np.float32).min, np.float32)])     # nothing but the mask's value: lse cannot hold it
+    ids = np.array([3, 1, -100, 5, -100, 4, 2])
+    g = np.array([1, -2, 3, 1, 1, 0, 1], np.float32)
+    h = np.array([0.5, 0.25, 0, 0, 0, 0, 0], np.float32)
+    out = RT.token_log_probs(client, client.upload(x), client.upload(ids))
+    d = client.read(RT.token_log_probs_backward(client, client.upload(x), client.upload(ids), out[1], out[2], client.upload(g), client.upload(h)))
+    want = R.scores_gradient(x[:2], ids[:2], 1.0, -100, g[:2], h[:2])
+    assert np.abs(d[:2] - want).max() <= 1e-5 and not d[0, 10:].any() and not d[1, ::2].any()
+    assert not d[2].any() and np.isnan(d[3]).all() and not d[4].any() and not d[5].any() and np.isnan(d[6]).all()
+
+
+def test_synchronous_context_reports_a_bad_id():
+    """The error of an id outside the vocabulary, in a process of its own: a context is synchronous for its whole life."""
+    import subprocess
+    import sys
+    code = ("import numpy as np\n"
+            "from rust_ascend_b200 import B200Runtime as RT, InvalidTensor, RuntimeOptions\n"
+            "c = RT.client(RT.initialize_exclusive(RuntimeOptions(0, True)))\n"
+            "x = c.upload(np.zeros((2, 50), np.float32))\n"
+            "RT.token_log_probs(c, x, c.upload(np.array([3, -100])))\n"
+            "try:\n    RT.token_log_probs(c, x, c.upload(np.array([50, 1])))\n"
+            "except InvalidTensor as e:\n    print('refused:', e)\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "refused: token log probabilities: an id is outside" in r.stdout, r.stdout + r.stderr
