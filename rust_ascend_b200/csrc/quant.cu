@@ -5,9 +5,11 @@
 // whole row, so max|y| = r max|s w| and y / scale = (s w) (127 / max|s w|): the quantised values do not need r at all, and one
 // reduction (the sum of squares beside the maximum) is enough where a norm followed by a quantisation has two.
 //
-// These kernels are HBM-bound.  One group of warps owns a row and keeps it in registers between the reduction and the store
-// (ITEMS vectors a thread); what a group cannot hold is read again, which hits L2.
+// These kernels are HBM-bound.  A group of warps owns a row and keeps it in shared memory between the reduction and the store; what
+// does not fit is read again, which hits L2.
 #include "common.cuh"
+
+#include <type_traits>
 
 namespace {
 
@@ -21,30 +23,120 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ bf from_f32<bf>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// BYTES-wide loads and stores of VEC elements; VEC * sizeof(T) is 1, 2, 4, 8, 16 or 32 bytes and the address is aligned to
-// min(that, 16).
+// VEC neighbouring elements: VEC * sizeof(T) is a power of two up to 32 bytes, and addresses are aligned to it or to 16.
 template <typename T, int VEC> struct __align__(VEC * sizeof(T) > 16 ? 16 : VEC * sizeof(T)) Pack { T v[VEC]; };
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load(const T* p, float (&v)[VEC]) {
-    const Pack<T, VEC> t = *reinterpret_cast<const Pack<T, VEC>*>(p);
+// A vector that nothing writes while the kernel runs: its load may move in front of stores.
+template <typename P> __device__ __forceinline__ P constant(const P* at) {
+    P p;
+    if constexpr (sizeof(P) % 16 == 0) {
+        uint4 t[sizeof(P) / 16];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = to_f32(t.v[j]);
+        for (int i = 0; i < (int)(sizeof(P) / 16); ++i) t[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
+        memcpy(&p, t, sizeof(P));
+    } else if constexpr (sizeof(P) == 8) { const uint2 t = __ldg(reinterpret_cast<const uint2*>(at)); memcpy(&p, &t, 8); }
+    else if constexpr (sizeof(P) == 4) { const uint32_t t = __ldg(reinterpret_cast<const uint32_t*>(at)); memcpy(&p, &t, 4); }
+    else { const uint16_t t = __ldg(reinterpret_cast<const uint16_t*>(at)); memcpy(&p, &t, 2); }
+    return p;
+}
+
+// Two FP32 operations in one instruction, each rounded as the single one is.
+__device__ __forceinline__ void mul2(float& a, float& b, float x, float y) {
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(a), "+f"(b) : "f"(x), "f"(y));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(a), "+f"(b) : "f"(x), "f"(y));
+}
+// (c, d) += (a * x, b * y)
+__device__ __forceinline__ void fma2(float& c, float& d, float a, float b, float x, float y) {
+    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 r, {%0, %1};\n\tfma.rn.f32x2 r, p, q, r;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "+f"(c), "+f"(d) : "f"(a), "f"(b), "f"(x), "f"(y));
+}
+// max(m, |a|, |b|), NaN if any of them is.
+__device__ __forceinline__ float max_abs(float m, float a, float b) { float d; asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(a), "f"(b)); return d; }
+
+// Elements widened to FP32; BF16 pairs by moving the bits.
+template <typename T, int VEC>
+__device__ __forceinline__ void widen(const Pack<T, VEC>& p, float (&v)[VEC]) {
+    if constexpr (VEC == 1 || sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = to_f32(p.v[j]);
+    } else {
+        uint32_t w[VEC / 2];
+        memcpy(w, &p, sizeof(w));
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+            if constexpr (std::is_same<T, bf>::value) { v[2 * j] = __uint_as_float(w[j] << 16); v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
+            else { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j])); v[2 * j] = f.x; v[2 * j + 1] = f.y; }
+        }
+    }
 }
 template <typename T, int VEC>
-__device__ __forceinline__ void store(T* p, const float (&v)[VEC]) {
-    Pack<T, VEC> t;
+__device__ __forceinline__ Pack<T, VEC> narrow(const float (&v)[VEC]) {
+    Pack<T, VEC> p;
+    if constexpr (VEC == 1 || sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) t.v[j] = from_f32<T>(v[j]);
-    *reinterpret_cast<Pack<T, VEC>*>(p) = t;
+        for (int j = 0; j < VEC; ++j) p.v[j] = from_f32<T>(v[j]);
+    } else {
+        uint32_t w[VEC / 2];
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+            if constexpr (std::is_same<T, bf>::value) { const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]); w[j] = *reinterpret_cast<const uint32_t*>(&h); }
+            else { const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]); w[j] = *reinterpret_cast<const uint32_t*>(&h); }
+        }
+        memcpy(&p, w, sizeof(w));
+    }
+    return p;
+}
+// a + b in the storage type.  The exact sum rounded once equals the FP32 sum rounded again: FP32 holds the sum of two 16-bit values
+// exactly unless their exponents are so far apart that the small one cannot reach the border between two results.
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> sum_of(const Pack<T, VEC>& a, const Pack<T, VEC>& b) {
+    Pack<T, VEC> p;
+    if constexpr (sizeof(T) == 4 || VEC == 1) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) p.v[j] = from_f32<T>(__fadd_rn(to_f32(a.v[j]), to_f32(b.v[j])));
+    } else {
+        uint32_t x[VEC / 2], y[VEC / 2];
+        memcpy(x, &a, sizeof(x)); memcpy(y, &b, sizeof(y));
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+            if constexpr (std::is_same<T, bf>::value) { const __nv_bfloat162 h = __hadd2_rn(*reinterpret_cast<__nv_bfloat162*>(&x[j]), *reinterpret_cast<__nv_bfloat162*>(&y[j])); x[j] = *reinterpret_cast<const uint32_t*>(&h); }
+            else { const __half2 h = __hadd2_rn(*reinterpret_cast<__half2*>(&x[j]), *reinterpret_cast<__half2*>(&y[j])); x[j] = *reinterpret_cast<const uint32_t*>(&h); }
+        }
+        memcpy(&p, x, sizeof(x));
+    }
+    return p;
 }
 // rint(v * c) as bytes: adding 1.5 * 2^23 leaves the integer in the low bits of the sum, rounded once (|v * c| <= 128).
 template <int VEC>
-__device__ __forceinline__ void store_i8(int8_t* p, const float (&v)[VEC], float c, bool bad) {
-    Pack<int8_t, VEC> t;
+__device__ __forceinline__ Pack<int8_t, VEC> to_bytes(const float (&v)[VEC], float c) {
+    constexpr float MAGIC = 12582912.0f;
+    Pack<int8_t, VEC> p;
+    if constexpr (VEC % 2 != 0) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) t.v[j] = bad ? (int8_t)0 : (int8_t)__float_as_uint(__fmaf_rn(v[j], c, 12582912.0f));
-    *reinterpret_cast<Pack<int8_t, VEC>*>(p) = t;
+        for (int j = 0; j < VEC; ++j) p.v[j] = (int8_t)__float_as_uint(__fmaf_rn(v[j], c, MAGIC));
+    } else {
+        uint32_t u[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            float lo = MAGIC, hi = MAGIC;
+            fma2(lo, hi, v[j], v[j + 1], c, c);
+            u[j] = __float_as_uint(lo); u[j + 1] = __float_as_uint(hi);
+        }
+        uint16_t h[VEC / 2];
+        uint32_t w[(VEC + 3) / 4];
+        if constexpr (VEC % 4 == 0) {
+#pragma unroll
+            for (int j = 0; j < VEC; j += 4) w[j / 4] = __byte_perm(__byte_perm(u[j], u[j + 1], 0x0040), __byte_perm(u[j + 2], u[j + 3], 0x0040), 0x5410);
+            memcpy(&p, w, VEC);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; j += 2) h[j / 2] = (uint16_t)__byte_perm(u[j], u[j + 1], 0x0040);
+            memcpy(&p, h, VEC);
+        }
+    }
+    return p;
 }
 
 enum Mode { PLAIN = 0, GATED = 1, NORM = 2, ADD_NORM = 3 };
@@ -53,176 +145,303 @@ struct QuantArgs {
     const void* x; uint64_t ldx;
     const void* other; uint64_t ldo;     // GATED: up; ADD_NORM: delta
     const void* w; void* x_out; int8_t* q; float* scales;
-    uint64_t rows; uint32_t width; uint32_t warps;   // warps that share a row
+    uint64_t rows; uint32_t width;
+    uint32_t warps;                      // warps that share a row
+    uint32_t held;                       // vectors of a row that fit its shared memory
+    uint32_t row_bytes;                  // shared memory of a row
     float eps;
 };
 
-// SiLU with one exponential and one reciprocal: x / (1 + exp(-x)).  For x below -88 the exponential overflows and the quotient is
-// the -0 that the limit has; an infinite or NaN x gives NaN or infinity, which marks the row.
-__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
-
-// Folds one vector into the two row statistics and leaves in v what the quantisation multiplies by one factor: y itself, or s * w.
-template <int MODE, int VEC>
-__device__ __forceinline__ void fold(float (&v)[VEC], const float (&w)[VEC], float& sum, uint32_t& most) {
+// SiLU(x) u = x u / (1 + 2^(-x log2 e)): one exponential and one reciprocal.  From x = -87.3 on down the reciprocal's argument leaves
+// the normal range and the result is -0; an infinite or NaN x gives NaN or infinity, which marks the row.
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float rcp(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+template <int VEC>
+__device__ __forceinline__ void silu_mul(float (&x)[VEC], const float (&u)[VEC]) {
+    constexpr float LOG2E = 1.44269504088896340736f;
+    if constexpr (VEC % 2 != 0) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        if (MODE == NORM || MODE == ADD_NORM) { sum = __fmaf_rn(v[j], v[j], sum); v[j] = __fmul_rn(v[j], w[j]); }
-        // magnitudes compare as integers, and in that order NaN lies above infinity, so neither is lost
-        const uint32_t bits = __float_as_uint(v[j]) & 0x7fffffffu;
-        most = most > bits ? most : bits;
+        for (int j = 0; j < VEC; ++j) x[j] = __fmul_rn(__fmul_rn(x[j], rcp(1.0f + ex2(x[j] * -LOG2E))), u[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            float e = x[j], f = x[j + 1];
+            mul2(e, f, -LOG2E, -LOG2E);
+            e = ex2(e); f = ex2(f);
+            add2(e, f, 1.0f, 1.0f);
+            mul2(x[j], x[j + 1], rcp(e), rcp(f));
+            mul2(x[j], x[j + 1], u[j], u[j + 1]);
+        }
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void times(float (&x)[VEC], const float (&w)[VEC]) {
+    if constexpr (VEC % 2 != 0) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[j] = __fmul_rn(x[j], w[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) mul2(x[j], x[j + 1], w[j], w[j + 1]);
     }
 }
 
-// `warps` whole warps share a row; a block holds blockDim.x / (32 warps) rows at a time, each with its own named
-// barrier, so rows of one block do not wait for each other.
-template <typename T, typename TW, int MODE, int VEC, int ITEMS>
-__global__ void __launch_bounds__(1024) quant_rows_kernel(const QuantArgs a) {
-    __shared__ float s_sum[32];
-    __shared__ uint32_t s_most[32];
+// A row between its two passes, in shared memory that only the thread which wrote it reads: the FP32 products where SiLU went
+// into them, the storage type's own values otherwise (the sum of a residual is rounded to it, so nothing is lost).
+// 32-byte vectors are kept as two planes of 16 bytes, so that neighbouring lanes stay on neighbouring banks.
+template <typename H, int VEC> struct Held {
+    static constexpr int PIECE = VEC * sizeof(H) > 16 ? 16 / sizeof(H) : VEC, PIECES = VEC / PIECE;
+    typedef Pack<H, PIECE> Piece;
+    static __device__ __forceinline__ void put(void* base, uint32_t held, uint32_t i, const Pack<H, VEC>& p) {
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) {
+            Piece part;
+#pragma unroll
+            for (int j = 0; j < PIECE; ++j) part.v[j] = p.v[c * PIECE + j];
+            static_cast<Piece*>(base)[c * held + i] = part;
+        }
+    }
+    static __device__ __forceinline__ Pack<H, VEC> get(const void* base, uint32_t held, uint32_t i) {
+        Pack<H, VEC> p;
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) {
+            const Piece part = static_cast<const Piece*>(base)[c * held + i];
+#pragma unroll
+            for (int j = 0; j < PIECE; ++j) p.v[c * PIECE + j] = part.v[j];
+        }
+        return p;
+    }
+};
+
+// `warps` whole warps share a row: the whole block, or one warp where that is enough (a block then holds eight rows, which do not
+// wait for each other).  Everything that the threads of a row compute alike is kept to one division: the root and the scale are the
+// first thread's business.
+template <typename T, typename TW, int MODE, int VEC, int UNROLL>
+__global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
+    constexpr bool NORMS = MODE == NORM || MODE == ADD_NORM, TWO = MODE == GATED || MODE == ADD_NORM;
+    typedef typename std::conditional<MODE == GATED, float, T>::type H;
+    typedef Held<H, VEC> Hold;
+    typedef Pack<T, VEC> In;
+    typedef Pack<TW, VEC> Weight;
+    typedef Pack<int8_t, VEC> Bytes;
+    extern __shared__ __align__(16) uint8_t s_rows[];
+    __shared__ float s_sum[16], s_most[16];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t group = warp / a.warps, groups = (blockDim.x >> 5) / a.warps, first_warp = group * a.warps;
     const uint32_t threads = a.warps * 32, tid = threadIdx.x - first_warp * 32;
     const uint32_t vectors = a.width / VEC;            // VEC divides the width
-    constexpr bool NORMS = MODE == NORM || MODE == ADD_NORM;
-    const T* other = static_cast<const T*>(a.other);
-    const TW* weight = static_cast<const TW*>(a.w);
+    void* mine = s_rows + (size_t)group * a.row_bytes;
+    const Weight* weight = static_cast<const Weight*>(a.w);
     for (uint64_t row = (uint64_t)blockIdx.x * groups + group; row < a.rows; row += (uint64_t)gridDim.x * groups) {
-        const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-        const T* o = other + row * a.ldo;
-        T* xo = static_cast<T*>(a.x_out) + row * a.width;
-        float v[ITEMS][VEC];
-        float sum = 0.f;
-        uint32_t most = 0;
-        // y, or s * w, of vector i; the sum of a residual is stored the first time it is formed and read back after that
-        auto fetch = [&](uint32_t i, float (&y)[VEC], float& acc, uint32_t& top, bool again) {
-            float second[VEC];
-            if (MODE == ADD_NORM && again) load<T, VEC>(xo + (size_t)i * VEC, y);
-            else load<T, VEC>(x + (size_t)i * VEC, y);
-            if (MODE == GATED || (MODE == ADD_NORM && !again)) load<T, VEC>(o + (size_t)i * VEC, second);
-            float w[VEC];
-            if (NORMS) load<TW, VEC>(weight + (size_t)i * VEC, w);
-            if (MODE == GATED) {
+        const In* x = reinterpret_cast<const In*>(static_cast<const T*>(a.x) + row * a.ldx);
+        const In* o = reinterpret_cast<const In*>(static_cast<const T*>(a.other) + row * a.ldo);
+        In* xo = reinterpret_cast<In*>(static_cast<T*>(a.x_out) + row * a.width);
+        Bytes* q = reinterpret_cast<Bytes*>(a.q + row * a.width);
+        float sum0 = 0.f, sum1 = 0.f, most = 0.f;
+        auto chunk = [&](uint32_t base, auto whole) {
+            In in[UNROLL], in2[TWO ? UNROLL : 1];
+            Weight wt[NORMS ? UNROLL : 1];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) y[j] = __fmul_rn(silu(y[j]), second[j]);
+            for (int u = 0; u < UNROLL; ++u) {
+                const uint32_t i = base + u * threads;
+                const uint32_t at = decltype(whole)::value || i < vectors ? i : vectors - 1;      // behind the row: the last vector again, not used
+                in[u] = x[at];
+                if (TWO) in2[TWO ? u : 0] = o[at];
+                if (NORMS) wt[NORMS ? u : 0] = constant(weight + at);
             }
-            if (MODE == ADD_NORM && !again) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) y[j] = to_f32(from_f32<T>(__fadd_rn(y[j], second[j])));
-                store<T, VEC>(xo + (size_t)i * VEC, y);
+            for (int u = 0; u < UNROLL; ++u) {
+                const uint32_t i = base + u * threads;
+                if (!decltype(whole)::value && i >= vectors) break;
+                float v[VEC];
+                [[maybe_unused]] float w[VEC];
+                if constexpr (MODE == ADD_NORM) { in[u] = sum_of<T, VEC>(in[u], in2[u]); xo[i] = in[u]; }
+                widen<T, VEC>(in[u], v);
+                if constexpr (MODE == GATED) { widen<T, VEC>(in2[u], w); silu_mul<VEC>(v, w); if (i < a.held) Hold::put(mine, a.held, i, narrow<float, VEC>(v)); }
+                else if (i < a.held) Hold::put(mine, a.held, i, in[u]);
+                if constexpr (NORMS) {
+                    if constexpr (VEC % 2 != 0) sum0 = __fmaf_rn(v[0], v[0], sum0);
+                    else {
+#pragma unroll
+                        for (int j = 0; j < VEC; j += 2) fma2(sum0, sum1, v[j], v[j + 1], v[j], v[j + 1]);
+                    }
+                    widen<TW, VEC>(wt[u], w);
+                    times<VEC>(v, w);
+                }
+                if constexpr (VEC % 2 != 0) most = max_abs(most, v[0], 0.f);
+                else {
+#pragma unroll
+                    for (int j = 0; j < VEC; j += 2) most = max_abs(most, v[j], v[j + 1]);
+                }
             }
-            fold<MODE, VEC>(y, w, acc, top);
         };
-#pragma unroll
-        for (int k = 0; k < ITEMS; ++k) {
-            const uint32_t i = k * threads + tid;
-            if (i < vectors) fetch(i, v[k], sum, most, false);
-        }
-        for (uint32_t i = ITEMS * threads + tid; i < vectors; i += threads) { float y[VEC]; fetch(i, y, sum, most, false); }
+        uint32_t base = tid;
+        for (; base + (UNROLL - 1) * threads < vectors; base += UNROLL * threads) chunk(base, std::true_type());
+        if (base < vectors) chunk(base, std::false_type());
 
-        most = __reduce_max_sync(0xffffffffu, most);
+        // magnitudes compare as integers, and in that order NaN lies above infinity
+        uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+        float sum = sum0 + sum1;
         if (NORMS) {
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         }
         if (a.warps > 1) {
             // a row's partial results: written, read after the first barrier, and not overwritten before the second
-            if (lane == 0) { s_sum[warp] = sum; s_most[warp] = most; }
-            asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
-            const uint32_t from = first_warp + (lane < a.warps ? lane : 0);
-            most = __reduce_max_sync(0xffffffffu, s_most[from]);
+            if (lane == 0) { s_sum[warp] = sum; s_most[warp] = __uint_as_float(bits); }
+            __syncthreads();
+            bits = __reduce_max_sync(0xffffffffu, __float_as_uint(s_most[lane < a.warps ? lane : 0]));
             if (NORMS) {
-                sum = lane < a.warps ? s_sum[from] : 0.f;
-#pragma unroll
-                for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                sum = 0.f;
+#pragma unroll 4
+                for (uint32_t i = 0; i < a.warps; ++i) sum += s_sum[i];
             }
-            asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
+            if (gridDim.x < a.rows) __syncthreads();
         }
-        const bool bad = most >= 0x7f800000u || (NORMS && sum != sum);
-        const float a_max = __uint_as_float(most);
-        const float r = NORMS ? __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)a.width), a.eps))) : 1.0f;
-        const float wanted = __fdiv_rn(__fmul_rn(r, a_max), 127.0f);
+        const bool bad = bits >= 0x7f800000u || (NORMS && sum != sum);
+        const float a_max = __uint_as_float(bits);
         const float least = 1.17549435e-38f;           // 2^-126
-        const bool tiny = wanted < least;
-        // The factor of a very small row would leave FP32's range: there the values are raised by 2^96 (exactly) first.
-        const bool small = a_max < 1e-30f;
-        const float c = tiny ? __fmul_rn(r, small ? 1073741824.0f : 8.5070592e37f)                    // r / 2^-126, over 2^96 where raised
-                             : __fdiv_rn(127.0f, small ? __fmul_rn(a_max, 7.9228163e28f) : a_max);
-        auto raise = [&](float (&y)[VEC]) {
-            if (!small) return;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) y[j] = __fmul_rn(y[j], 7.9228163e28f);
-        };
-        if (tid == 0) a.scales[row] = bad ? __int_as_float(0x7fc00000) : (tiny ? least : wanted);
-        int8_t* q = a.q + row * a.width;
-#pragma unroll
-        for (int k = 0; k < ITEMS; ++k) {
-            const uint32_t i = k * threads + tid;
-            if (i < vectors) { raise(v[k]); store_i8<VEC>(q + (size_t)i * VEC, v[k], c, bad); }
+        float c = __fdiv_rn(127.0f, a_max);
+        // Rows so small (or a norm so large) that the scale may end at 2^-126, and the factor leave FP32's range: there the values
+        // are raised by 2^96 (exactly) first.
+        const bool small = a_max < 1e-16f || (NORMS && sum > 3.4028235e38f);
+        if (tid == 0 || small) {
+            const float r = NORMS ? __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)a.width), a.eps))) : 1.0f;
+            const float wanted = __fdiv_rn(__fmul_rn(r, a_max), 127.0f);
+            const bool tiny = wanted < least, raised = a_max < 1e-16f;
+            if (tid == 0) a.scales[row] = bad ? __int_as_float(0x7fc00000) : (tiny ? least : wanted);
+            if (small) {
+                c = tiny ? __fmul_rn(r, 1073741824.0f) : __fdiv_rn(127.0f, __fmul_rn(a_max, 7.9228163e28f));       // r 2^126, or 127 / max, over 2^96
+                if (!raised) c = __fmul_rn(c, 7.9228163e28f);
+            }
         }
-        for (uint32_t i = ITEMS * threads + tid; i < vectors; i += threads) {
-            float y[VEC], unused = 0.f; uint32_t none = 0;
-            fetch(i, y, unused, none, true);
-            raise(y);
-            store_i8<VEC>(q + (size_t)i * VEC, y, c, bad);
+        const bool raise = a_max < 1e-16f;
+        auto finish = [&](uint32_t i, auto plain) {
+            float v[VEC];
+            [[maybe_unused]] float w[VEC];
+            if (i < a.held) widen<H, VEC>(Hold::get(mine, a.held, i), v);
+            else {
+                widen<T, VEC>(MODE == ADD_NORM ? xo[i] : x[i], v);
+                if constexpr (MODE == GATED) { widen<T, VEC>(o[i], w); silu_mul<VEC>(v, w); }
+            }
+            if constexpr (NORMS) { widen<TW, VEC>(constant(weight + i), w); times<VEC>(v, w); }
+            if (!decltype(plain)::value) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] = bad ? 0.f : (raise ? __fmul_rn(v[j], 7.9228163e28f) : v[j]);
+            }
+            q[i] = to_bytes<VEC>(v, !decltype(plain)::value && bad ? 0.f : c);
+        };
+        if (!bad && !small) {
+#pragma unroll 4
+            for (uint32_t i = tid; i < vectors; i += threads) finish(i, std::true_type());
+        } else {
+#pragma unroll 1
+            for (uint32_t i = tid; i < vectors; i += threads) finish(i, std::false_type());
         }
     }
 }
 
-template <typename T, typename TW, int MODE, int VEC, int ITEMS>
+constexpr uint32_t ROW_SMEM = 96 * 1024;     // shared memory a row may take: at least two rows an SM
+
+template <typename T, typename TW, int MODE, int VEC, int UNROLL>
 int32_t launch(rb_ctx* ctx, QuantArgs a, const char* what) {
+    typedef typename std::conditional<MODE == GATED, float, T>::type H;
+    static std::once_flag once;
+    static cudaError_t configured = cudaSuccess;
+    std::call_once(once, [] { configured = cudaFuncSetAttribute(quant_rows_kernel<T, TW, MODE, VEC, UNROLL>, cudaFuncAttributeMaxDynamicSharedMemorySize, ROW_SMEM); });
+    if (configured != cudaSuccess) return rb::fail(RB_STATUS, "%s: cudaFuncSetAttribute failed with CUDA status %d (%s)", what, (int)configured, cudaGetErrorString(configured));
     const uint32_t vectors = a.width / VEC;
-    uint32_t warps = (vectors + ITEMS * 32 - 1) / (ITEMS * 32);
-    if (warps < 1) warps = 1;
-    if (warps > 32) warps = 32;
+    // Many rows: a few vectors a thread, so that what all threads of a row do alike weighs little and several rows share an SM (one's
+    // loads run under another's reduction).  8192 x 4096 BF16 with residual: 37.1 us at four vectors a thread, 42.2 at two, 70 at one.
+    // SiLU over 4096 x 14336 BF16: 53.9 us at eight, 57.3 at four.  Few rows: latency, so one vector a thread where that fits.
+    const uint32_t wanted = a.rows <= (uint64_t)ctx->sm_count ? 1 : (VEC == 1 ? 20 : (MODE == GATED ? 8 : 4));
+    uint32_t warps = (vectors + wanted * 32 - 1) / (wanted * 32);
+    if (warps > 16) warps = 16;
     a.warps = warps;
-    const uint32_t groups = warps >= 8 ? 1 : 8 / warps;            // blocks of about 256 threads for narrow rows; at most 8 groups: barriers 1..8
-    const uint64_t blocks = (a.rows + groups - 1) / groups, cap = (uint64_t)ctx->sm_count * 32;
-    quant_rows_kernel<T, TW, MODE, VEC, ITEMS><<<(unsigned)(blocks < cap ? blocks : cap), groups * warps * 32, 0, ctx->stream>>>(a);
+    const uint32_t groups = warps == 1 ? 8 : 1;
+    const uint32_t vector_bytes = VEC * sizeof(H), most_held = ROW_SMEM / groups / vector_bytes;
+    a.held = vectors < most_held ? vectors : most_held;
+    a.row_bytes = (a.held * vector_bytes + 15) & ~15u;
+    if (a.row_bytes * groups > ROW_SMEM) { a.held -= 16; a.row_bytes = (a.held * vector_bytes + 15) & ~15u; }
+    const uint64_t blocks = (a.rows + groups - 1) / groups, cap = 1u << 30;
+    quant_rows_kernel<T, TW, MODE, VEC, UNROLL><<<(unsigned)(blocks < cap ? blocks : cap), groups * warps * 32, a.row_bytes * groups, ctx->stream>>>(a);
     return rb::after_launch(ctx, what);
 }
 
-// 16-byte vectors where every row of every operand starts on one; single elements otherwise.
+// The widest vectors on which every row of every operand starts: 16 bytes, 8 bytes, or single elements.
 template <typename T, typename TW, int MODE>
 int32_t dispatch(rb_ctx* ctx, const QuantArgs& a, const char* what) {
-    constexpr int VEC = 16 / sizeof(T);
-    auto fits = [](const void* p, uint64_t ld, size_t es, size_t bytes) { return p == nullptr || ((uintptr_t)p % bytes == 0 && ld * es % bytes == 0); };
-    const bool wide = a.width % VEC == 0 && fits(a.x, a.ldx, sizeof(T), 16) && fits(a.other, a.ldo, sizeof(T), 16) && fits(a.w, 0, sizeof(TW), 16) &&
-                      fits(a.x_out, a.width, sizeof(T), 16) && fits(a.q, a.width, 1, VEC);
-    if (wide) return launch<T, TW, MODE, VEC, 2>(ctx, a, what);
-    return launch<T, TW, MODE, 1, 8>(ctx, a, what);
+    constexpr int FULL = 16 / sizeof(T), HALF = FULL / 2;
+    auto fits = [&](int vec) {
+        auto on = [](const void* p, uint64_t ld, size_t es, size_t bytes) { return p == nullptr || ((uintptr_t)p % bytes == 0 && ld * es % bytes == 0); };
+        const size_t b = vec * sizeof(T), wb = vec * sizeof(TW) > 16 ? 16 : vec * sizeof(TW);
+        return a.width % vec == 0 && on(a.x, a.ldx, sizeof(T), b) && on(a.other, a.ldo, sizeof(T), b) && on(a.w, 0, sizeof(TW), wb) &&
+               on(a.x_out, a.width, sizeof(T), b) && on(a.q, a.width, 1, vec);
+    };
+    if (fits(FULL)) return launch<T, TW, MODE, FULL, MODE == ADD_NORM ? 2 : 4>(ctx, a, what);
+    if (fits(HALF)) return launch<T, TW, MODE, HALF, 4>(ctx, a, what);
+    return launch<T, TW, MODE, 1, 4>(ctx, a, what);
 }
 
-// y = q * scale on flat 16-element vectors (q and y are contiguous, so vectors stay aligned whatever the width); the row of a
+// Division by a number that is known on the host: n / d = (umulhi(n, m) + n) / 2^s for d < 2^31, with m = floor(2^32 (2^s - d) / d) + 1
+// and s = ceil(log2 d) (Granlund and Montgomery, 1994), the sum taken in 33 bits by halving.
+struct Divisor { uint32_t d, m, s; };
+__host__ Divisor divisor(uint32_t d) {
+    uint32_t s = 0;
+    while ((uint64_t(1) << s) < d) ++s;
+    return {d, (uint32_t)(((uint64_t(1) << 32) * ((uint64_t(1) << s) - d)) / d + 1), s};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t n, const Divisor& v) {
+    const uint32_t t = __umulhi(n, v.m);
+    return v.s == 0 ? n : (t + ((n - t) >> 1)) >> (v.s - 1);
+}
+__device__ __forceinline__ uint64_t divide(uint64_t n, const Divisor& v) { return n / v.d; }
+
+// y = q * scale on flat vectors of 16 bytes of y (q and y are contiguous, so they stay aligned whatever the width); the row of a
 // vector's first element comes from one division, a row's end inside the vector steps to the next scale.
-template <typename T>
-__global__ void __launch_bounds__(256) dequant_kernel(const int8_t* q, const float* scales, T* y, uint64_t total, uint32_t width) {
-    const uint64_t vectors = total / 16, stride = (uint64_t)gridDim.x * blockDim.x;
-    for (uint64_t v = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; v < vectors; v += stride) {
-        const uint64_t at = v * 16;
-        uint64_t row = total <= 0xffffffffull ? (uint64_t)((uint32_t)at / width) : at / width;
-        uint32_t col = (uint32_t)(at - row * width);
-        const uint4 b = __ldcs(reinterpret_cast<const uint4*>(q + at));
-        float s = __ldg(scales + row);
-        const uint32_t word[4] = {b.x, b.y, b.z, b.w};
-        float o[16];
+template <typename T, typename Index>
+__global__ void __launch_bounds__(256) dequant_kernel(const int8_t* q, const float* scales, T* y, uint64_t total, uint32_t width, const Divisor by_width) {
+    constexpr int PER = 16 / sizeof(T), UNROLL = 32 / PER;         // 32 elements a thread
+    typedef Pack<int8_t, PER> Bytes;
+    const Index vectors = (Index)(total / PER), base = (Index)blockIdx.x * 256 * UNROLL + threadIdx.x;
+    Bytes b[UNROLL];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+    for (int u = 0; u < UNROLL; ++u) if (base + u * 256 < vectors) b[u] = reinterpret_cast<const Bytes*>(q)[base + u * 256];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const Index v = base + u * 256;
+        if (v >= vectors) break;
+        const Index row = divide(v * PER, by_width);
+        uint32_t col = (uint32_t)(v * PER - row * (Index)width);
+        const float s = __ldg(scales + row);
+        float f[PER], by[PER];
+        uint32_t word[PER / 4];
+        memcpy(word, &b[u], PER);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
             // byte + 128 as the low bits of 2^23, so that the difference is the signed byte, exactly
-            const float f = __uint_as_float(__byte_perm(word[j / 4] ^ 0x80808080u, 0x4b000000u, 0x7650 | (j % 4))) - 8388736.0f;
-            o[j] = __fmul_rn(f, s);
-            if (j < 15 && ++col == width) { col = 0; ++row; s = __ldg(scales + row); }
+            f[j] = __uint_as_float(__byte_perm(word[j / 4] ^ 0x80808080u, 0x4b000000u, 0x7650 | (j % 4)));
+            by[j] = s;
         }
-        constexpr int PER = 16 / sizeof(T);
+        if (col + PER > width) {
+            Index r = row;
 #pragma unroll
-        for (int j = 0; j < 16; j += PER) {
-            float part[PER];
-#pragma unroll
-            for (int i = 0; i < PER; ++i) part[i] = o[j + i];
-            store<T, PER>(y + at + j, part);
+            for (int j = 1; j < PER; ++j) { if (++col == width) { col = 0; ++r; } by[j] = __ldg(scales + r); }
         }
+#pragma unroll
+        for (int j = 0; j < PER; j += 2) add2(f[j], f[j + 1], -8388736.0f, -8388736.0f);
+        times<PER>(f, by);
+        reinterpret_cast<Pack<T, PER>*>(y)[v] = narrow<T, PER>(f);
     }
-    const uint64_t tail = vectors * 16 + threadIdx.x;
-    if (blockIdx.x == 0 && threadIdx.x < 16 && tail < total) y[tail] = from_f32<T>(__fmul_rn((float)q[tail], scales[tail / width]));
+    const uint64_t tail = (uint64_t)vectors * PER + threadIdx.x;
+    if (blockIdx.x == 0 && threadIdx.x < PER && tail < total) y[tail] = from_f32<T>(__fmul_rn((float)q[tail], scales[tail / width]));
+}
+
+template <typename T>
+void launch_dequant(rb_ctx* ctx, const int8_t* q, const float* scales, void* y, uint64_t total, uint32_t width) {
+    const uint64_t blocks = (total + 8191) / 8192;
+    const unsigned grid = (unsigned)(blocks ? blocks : 1);
+    if (total <= 0xf0000000ull) dequant_kernel<T, uint32_t><<<grid, 256, 0, ctx->stream>>>(q, scales, (T*)y, total, width, divisor(width));
+    else dequant_kernel<T, uint64_t><<<grid, 256, 0, ctx->stream>>>(q, scales, (T*)y, total, width, divisor(width));
 }
 
 bool is_float(uint32_t dtype) { return dtype == RB_F32 || dtype == RB_BF16 || dtype == RB_F16; }
@@ -266,7 +485,7 @@ int32_t rb_rms_norm_quant(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* delt
     }
     if (rows == 0) return empty_call(ctx);
     DeviceGuard device(ctx);
-    QuantArgs a{px, width, pd, width, pw, pxo, (int8_t*)pq, (float*)ps, rows, (uint32_t)width, 0, eps};
+    QuantArgs a{px, width, pd, width, pw, pxo, (int8_t*)pq, (float*)ps, rows, (uint32_t)width, 0, 0, 0, eps};
 #define RB_NORM(T, TW) return delta ? dispatch<T, TW, ADD_NORM>(ctx, a, what) : dispatch<T, TW, NORM>(ctx, a, what)
     if (x->dtype == RB_F32) RB_NORM(float, float);
     if (x->dtype == RB_BF16 && weight->dtype == RB_BF16) RB_NORM(bf, bf);
@@ -293,7 +512,7 @@ int32_t rb_quantize_rows(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* up, c
     if (up) { RB_TRY(no_overlap(pq, n, ru.ptr, ru.extent_bytes, what)); RB_TRY(no_overlap(ps, sb, ru.ptr, ru.extent_bytes, what)); }
     if (rx.rows == 0) return empty_call(ctx);
     DeviceGuard device(ctx);
-    QuantArgs a{rx.ptr, rx.ld, ru.ptr, ru.ld, nullptr, nullptr, (int8_t*)pq, (float*)ps, rx.rows, (uint32_t)rx.width, 0, 0.f};
+    QuantArgs a{rx.ptr, rx.ld, ru.ptr, ru.ld, nullptr, nullptr, (int8_t*)pq, (float*)ps, rx.rows, (uint32_t)rx.width, 0, 0, 0, 0.f};
     if (x->dtype == RB_F32) return up ? dispatch<float, float, GATED>(ctx, a, what) : dispatch<float, float, PLAIN>(ctx, a, what);
     if (x->dtype == RB_BF16) return up ? dispatch<bf, bf, GATED>(ctx, a, what) : dispatch<bf, bf, PLAIN>(ctx, a, what);
     return up ? dispatch<__half, __half, GATED>(ctx, a, what) : dispatch<__half, __half, PLAIN>(ctx, a, what);
@@ -309,15 +528,13 @@ int32_t rb_dequantize_rows(rb_ctx* ctx, const rb_tensor* q, const rb_tensor* sca
     if (width == 0 || width > 0x7fffffffull) return fail(RB_INVALID_TENSOR, "%s requires a positive last dimension within INT32_MAX", what);
     RB_TRY(check_result(ctx, y, rows, q, scales, what, &pq, &ps));
     const uint64_t n = rows * width, yb = n * dtype_size(y->dtype);
+    if (n / 8192 > 0x7ffffff0ull) return fail(RB_INVALID_TENSOR, "%s: too many values for one launch", what);
     RB_TRY(no_overlap(py, yb, pq, n, what)); RB_TRY(no_overlap(py, yb, ps, rows * 4, what));
     if (rows == 0) return empty_call(ctx);
     DeviceGuard device(ctx);
-    const uint64_t blocks = (n / 16 + 255) / 256, cap = (uint64_t)ctx->sm_count * 16;
-    const unsigned grid = (unsigned)(blocks < 1 ? 1 : (blocks < cap ? blocks : cap));
-    const int8_t* in = (const int8_t*)pq; const float* s = (const float*)ps;
-    if (y->dtype == RB_F32) dequant_kernel<float><<<grid, 256, 0, ctx->stream>>>(in, s, (float*)py, n, (uint32_t)width);
-    else if (y->dtype == RB_BF16) dequant_kernel<bf><<<grid, 256, 0, ctx->stream>>>(in, s, (bf*)py, n, (uint32_t)width);
-    else dequant_kernel<__half><<<grid, 256, 0, ctx->stream>>>(in, s, (__half*)py, n, (uint32_t)width);
+    if (y->dtype == RB_F32) launch_dequant<float>(ctx, (const int8_t*)pq, (const float*)ps, py, n, (uint32_t)width);
+    else if (y->dtype == RB_BF16) launch_dequant<bf>(ctx, (const int8_t*)pq, (const float*)ps, py, n, (uint32_t)width);
+    else launch_dequant<__half>(ctx, (const int8_t*)pq, (const float*)ps, py, n, (uint32_t)width);
     return after_launch(ctx, what);
 }
 
