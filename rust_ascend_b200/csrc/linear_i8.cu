@@ -8,7 +8,8 @@
 // weights and pays for as many columns as there are tokens (16 at least), and an output row y[m, ..] is stored by neighbouring lanes,
 // so no N needs alignment.
 //
-// Two kernels:
+// Three kernels:
+//   * one to four tokens: a warp per weight row (or two), 16-byte loads and dot products of four bytes; no set-up but the launch.
 //   * few tokens: one tile of 128 weight rows x TOKENS tokens per cluster, K split over the cluster's CTAs so that all SMs stream
 //     weights; the parts are added through distributed shared memory.  Bound: the bytes of W.
 //   * many tokens: CTA pairs (cta_group::2) on 256 x 256 tiles, persistent, two accumulators in TMEM so that the store of one tile runs
@@ -32,8 +33,8 @@ constexpr int THREADS = 192;     // producer, issuer, four epilogue warps
 struct LinearParams {
     uint32_t m, n, num_kb;
     uint32_t tiles_t, tiles_n;       // token tiles, weight tiles
+    uint32_t tokens;                 // pair kernel: tokens of a whole tile, a multiple of 32 within 256
     uint32_t split, items;           // pair kernel: whole tiles, all work items (see rb_gemm_plan)
-    uint32_t out;                    // 0 BF16, 1 FP32, 2 FP16
     const float* sx; const float* sw; const float* bias;
     void* y;
     uint32_t* status;
@@ -67,29 +68,117 @@ __device__ __forceinline__ int32_t ld_cluster_s32(uint32_t addr) {
     int32_t v; asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory"); return v;
 }
 
-// One output value.
-__device__ __forceinline__ void put(const LinearParams& p, uint32_t token, uint32_t col, int32_t acc, float sx, float sw, float bias) {
-    float v = __fmul_rn(__int2float_rn(acc), __fmul_rn(sx, sw));
-    if (p.bias) v = __fadd_rn(v, bias);
-    const size_t at = (size_t)token * p.n + col;
-    if (p.out == 1) static_cast<float*>(p.y)[at] = v;
-    else if (p.out == 2) static_cast<__half*>(p.y)[at] = __float2half_rn(v);
-    else static_cast<bf*>(p.y)[at] = __float2bfloat16_rn(v);
+template <typename Out> __device__ __forceinline__ Out rounded(float v);
+template <> __device__ __forceinline__ float rounded<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf rounded<bf>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half rounded<__half>(float v) { return __float2half_rn(v); }
+
+// N tokens of one output column, `count` of which exist: y[(token + j) * n + col] for the sums acc[j].  sx: the tokens' scales in shared
+// memory.  Lanes are neighbouring columns, so each store is one row segment.  The whole block of values is formed before the first
+// store: a branch inside the loop costs the epilogue its instruction-level parallelism (measured: 16 us instead of 3 per 256 x 256 tile).
+template <typename Out, int N>
+__device__ __forceinline__ void put(const LinearParams& p, uint32_t token, uint32_t col, const uint32_t (&acc)[N], const float* sx, float sw, float bias, uint32_t count) {
+    float v[N];
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(sx + j);
+        v[j] = __fmul_rn(__int2float_rn((int32_t)acc[j]), __fmul_rn(s.x, sw));
+        v[j + 1] = __fmul_rn(__int2float_rn((int32_t)acc[j + 1]), __fmul_rn(s.y, sw));
+        v[j + 2] = __fmul_rn(__int2float_rn((int32_t)acc[j + 2]), __fmul_rn(s.z, sw));
+        v[j + 3] = __fmul_rn(__int2float_rn((int32_t)acc[j + 3]), __fmul_rn(s.w, sw));
+    }
+    if (p.bias) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], bias);
+    }
+    if (col >= p.n) return;
+    Out* at = static_cast<Out*>(p.y) + (size_t)token * p.n;
+    if (count >= (uint32_t)N) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) at[(size_t)j * p.n + col] = rounded<Out>(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) if ((uint32_t)j < count) at[(size_t)j * p.n + col] = rounded<Out>(v[j]);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Few tokens.  Stages are sized so that two CTAs share an SM (one streams while the other starts or stores); TOKENS = 256 takes the SM.
+// One to four tokens: bound by the bytes of W and, for small layers, by latency.  A warp reads R rows of W, so that a load of x (from
+// L1) serves R times, and has four to eight vectors of 16 bytes a lane in flight: the next round's loads leave before this round's
+// products.  6144 x 4096, one token: 5.9 us = 4.2 TB/s with the launch; 14336 x 4096: 10.8 us = 5.4 TB/s.
+template <typename Out, int M, int R>
+__global__ void __launch_bounds__(128) linear_i8_row_kernel(const int8_t* __restrict__ x, const int8_t* __restrict__ w, const LinearParams p, const uint32_t k) {
+    constexpr int UNROLL = 4 / R;
+    const uint32_t lane = threadIdx.x & 31, row0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * R;
+    if (row0 >= p.n) return;                            // a whole warp
+    const uint32_t vectors = k / 16;
+    const uint4* at[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) at[r] = reinterpret_cast<const uint4*>(w + (size_t)(row0 + r < p.n ? row0 + r : p.n - 1) * k);
+    auto load = [&](uint32_t base, uint4 (&a)[R][UNROLL]) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const uint32_t i = base + u * 32;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                a[r][u] = make_uint4(0, 0, 0, 0);       // behind the row: adds nothing
+                if (i < vectors) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a[r][u].x), "=r"(a[r][u].y), "=r"(a[r][u].z), "=r"(a[r][u].w) : "l"(at[r] + i));
+            }
+        }
+    };
+    int32_t acc[R][M] = {};
+    uint4 a[R][UNROLL], ahead[R][UNROLL];
+    load(lane, a);
+    load(lane + 32 * UNROLL, ahead);
+    for (uint32_t base = lane; base - lane < vectors; base += 32 * UNROLL) {      // the same number of rounds for every lane
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const uint32_t i = base + u * 32 < vectors ? base + u * 32 : 0;
+#pragma unroll
+            for (int t = 0; t < M; ++t) {
+                const uint4 b = __ldg(reinterpret_cast<const uint4*>(x + (size_t)((uint32_t)t < p.m ? t : 0) * k) + i);      // a missing token repeats the first
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    acc[r][t] = __dp4a((int)a[r][u].x, (int)b.x, acc[r][t]);
+                    acc[r][t] = __dp4a((int)a[r][u].y, (int)b.y, acc[r][t]);
+                    acc[r][t] = __dp4a((int)a[r][u].z, (int)b.z, acc[r][t]);
+                    acc[r][t] = __dp4a((int)a[r][u].w, (int)b.w, acc[r][t]);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) a[r][u] = ahead[r][u];
+        load(base + 64 * UNROLL, ahead);
+    }
+    // lane r * M + t ends with row r, token t
+    int32_t mine = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < M; ++t) { const int32_t sum = __reduce_add_sync(0xffffffffu, acc[r][t]); if (lane == (uint32_t)(r * M + t)) mine = sum; }
+    const uint32_t r = lane / M, t = lane - r * M, col = row0 + r;
+    if (r < (uint32_t)R && t < p.m && col < p.n) {
+        float v = __fmul_rn(__int2float_rn(mine), __fmul_rn(p.sx[t], p.sw[col]));
+        if (p.bias) v = __fadd_rn(v, p.bias[col]);
+        static_cast<Out*>(p.y)[(size_t)t * p.n + col] = rounded<Out>(v);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Few tokens.  Stages are sized so that two CTAs share an SM (one streams while the other starts or stores).
 template <int TOKENS> struct Few {
     static constexpr int B_BYTES = TOKENS * BK;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = TOKENS == 16 ? 6 : TOKENS == 32 ? 5 : TOKENS == 64 ? 4 : TOKENS == 128 ? 3 : 4;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*alignment*/ + 128 /*barriers*/;
+    static constexpr int STAGES = TOKENS == 16 ? 6 : TOKENS == 32 ? 5 : TOKENS == 64 ? 4 : 3;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*alignment*/ + 128 /*barriers*/ + TOKENS * 4 /*scales*/;
     static constexpr int TMEM_COLS = TOKENS < 32 ? 32 : TOKENS;
     static_assert(TOKENS * ROWS * 4 <= STAGES * STAGE_BYTES, "the parts of a split K are exchanged in the stage buffers");
 };
 
-template <int TOKENS>
-__global__ void __launch_bounds__(THREADS, TOKENS == 256 ? 1 : 2)
+template <typename Out, int TOKENS>
+__global__ void __launch_bounds__(THREADS, 2)
 linear_i8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LinearParams p) {
     using C = Few<TOKENS>;
     extern __shared__ uint8_t smem_raw[];
@@ -99,6 +188,7 @@ linear_i8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     uint64_t* done_bar = empty_bar + C::STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
     volatile uint32_t* abort_word = tmem_slot + 1;
+    float* sx = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES + 128);
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t parts; asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(parts));
@@ -106,15 +196,26 @@ linear_i8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     const uint32_t tile = blockIdx.x / parts, tn = tile / p.tiles_t, tt = tile - tn * p.tiles_t;   // neighbours share the weight rows
     const uint32_t row0 = tn * ROWS, token0 = tt * TOKENS;
     const uint32_t kb0 = (uint32_t)((uint64_t)p.num_kb * rank / parts), kb1 = (uint32_t)((uint64_t)p.num_kb * (rank + 1) / parts);
+    const uint32_t tokens = p.m - token0 < (uint32_t)TOKENS ? p.m - token0 : TOKENS;
 
+    auto fetch = [&](uint32_t kb, uint32_t stage) {
+        uint8_t* sa = smem + stage * C::STAGE_BYTES;
+        mbar_expect_tx(&full_bar[stage], C::STAGE_BYTES);
+        tma_load_2d(sa, &map_w, &full_bar[stage], (int32_t)(kb * BK), (int32_t)row0);
+        tma_load_2d(sa + A_BYTES, &map_x, &full_bar[stage], (int32_t)(kb * BK), (int32_t)token0);
+    };
+    // The first stages are on their way before anything else is set up: the thread that makes the barriers fills the ring.
+    const uint32_t ahead = kb1 - kb0 < (uint32_t)C::STAGES ? kb1 - kb0 : C::STAGES;
     if (threadIdx.x == 0) {
+        prefetch_tmap(&map_w); prefetch_tmap(&map_x);
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
         mbar_init(done_bar, 1);
         *abort_word = 0;
         fence_barrier_init();
-        prefetch_tmap(&map_w); prefetch_tmap(&map_x);
+        for (uint32_t i = 0; i < ahead; ++i) fetch(kb0 + i, i);
     }
     if (warp == 1) { tmem_alloc(tmem_slot, C::TMEM_COLS); tmem_relinquish(); }
+    for (uint32_t j = threadIdx.x; j < (uint32_t)TOKENS; j += THREADS) sx[j] = j < tokens ? p.sx[token0 + j] : 0.f;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -122,21 +223,15 @@ linear_i8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 
     bool ok = true;
     if (warp == 0) {
-        if (elect_one()) {
-            uint32_t stage = 0, phase = 0, armed = 0, armed_parity = 0;
-            for (uint32_t kb = kb0; kb < kb1; ++kb) {
-                if (!(ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_word))) break;
-                uint8_t* sa = smem + stage * C::STAGE_BYTES;
-                mbar_expect_tx(&full_bar[stage], C::STAGE_BYTES);
-                armed |= 1u << stage; armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
-                tma_load_2d(sa, &map_w, &full_bar[stage], (int32_t)(kb * BK), (int32_t)row0);
-                tma_load_2d(sa + A_BYTES, &map_x, &full_bar[stage], (int32_t)(kb * BK), (int32_t)token0);
+        if (threadIdx.x == 0) {
+            uint32_t stage = 0, phase = 0;           // the next fill of stage s waits for its (phase + 1)-th release
+            for (uint32_t kb = kb0 + ahead; kb < kb1; ++kb) {
+                if (!(ok = mbar_wait(&empty_bar[stage], phase, abort_word))) break;
+                fetch(kb, stage);
                 if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
             }
-            if (!ok)   // a wait ran out: let the copies this thread issued land before the CTA retires
-                for (int s = 0; s < C::STAGES; ++s)
-                    if (armed & (1u << s))
-                        for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(&full_bar[s], (armed_parity >> s) & 1u); ++i) {}
+            if (!ok)   // a wait ran out: a bounded time for the copies in flight to land before the CTA retires
+                for (uint32_t i = 0; i < (1u << 22); ++i) __nanosleep(32);
         }
     } else if (warp == 1) {
         if (elect_one()) {
@@ -155,23 +250,18 @@ linear_i8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         }
     } else {
         const uint32_t quarter = warp & 3, row = quarter * 32 + lane, col = row0 + row;
-        const uint32_t tokens = p.m - token0 < (uint32_t)TOKENS ? p.m - token0 : TOKENS;
         const float sw = col < p.n ? p.sw[col] : 0.f, bias = p.bias && col < p.n ? p.bias[col] : 0.f;
         ok = mbar_wait(done_bar, 0, abort_word);
         ok = __all_sync(0xffffffffu, ok);
+        int32_t* part = reinterpret_cast<int32_t*>(smem);       // [TOKENS][ROWS], over the stages: every product has been read
         if (ok) {
             tc_fence_after();
-            int32_t* part = reinterpret_cast<int32_t*>(smem);       // [TOKENS][ROWS], over the stages: every product has been read
             for (uint32_t c = 0; c < tokens; c += 16) {
                 uint32_t r[16];
                 tmem_ld_32x16(tmem + ((quarter * 32) << 16) + c, r);
                 tmem_wait_ld();
-                if (parts == 1) {
-                    if (col < p.n) {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) if (c + j < tokens) put(p, token0 + c + j, col, (int32_t)r[j], __ldg(p.sx + token0 + c + j), sw, bias);
-                    }
-                } else {
+                if (parts == 1) put<Out, 16>(p, token0 + c, col, r, sx + c, sw, bias, tokens - c);
+                else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) part[(c + j) * ROWS + row] = (int32_t)r[j];
                 }
@@ -179,16 +269,25 @@ linear_i8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             tc_fence_before();
         }
         if (parts > 1) {
-            // Every CTA of the cluster adds up its share of the tokens from all parts.  All threads of the cluster meet at the two
-            // barriers, whatever happened before; after a wait that ran out the sums are wrong and the status word says so.
+            // Every CTA of the cluster adds up its share of the tokens from all parts, in groups of four.  All threads of the cluster
+            // meet at the two barriers, whatever happened before; after a wait that ran out the sums are wrong and the status word
+            // says so.
+            __syncwarp();
             cluster_sync_all();
-            const uint32_t first = tokens * rank / parts, last = tokens * (rank + 1) / parts;
-            for (uint32_t t = first; t < last; ++t) {
-                int32_t acc = 0;
-                const uint32_t at = smem_u32(smem) + (t * ROWS + row) * 4;
-                for (uint32_t s = 0; s < parts; ++s) acc += ld_cluster_s32(mapa_shared(at, s));
-                if (col < p.n) put(p, token0 + t, col, acc, __ldg(p.sx + token0 + t), sw, bias);
+            const uint32_t groups = (tokens + 3) / 4, first = groups * rank / parts, last = groups * (rank + 1) / parts;
+#pragma unroll 2
+            for (uint32_t g = first; g < last; ++g) {
+                uint32_t acc[4] = {0, 0, 0, 0};
+                const uint32_t at = smem_u32(part) + (g * 4 * ROWS + row) * 4;
+#pragma unroll 4
+                for (uint32_t s = 0; s < parts; ++s) {
+                    const uint32_t from = mapa_shared(at, s);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[j] += (uint32_t)ld_cluster_s32(from + j * ROWS * 4);
+                }
+                put<Out, 4>(p, token0 + g * 4, col, acc, sx + g * 4, sw, bias, tokens - g * 4);
             }
+            __syncwarp();
             cluster_sync_all();      // nobody leaves while its part is being read
         }
     }
@@ -216,10 +315,11 @@ __device__ __forceinline__ Item item_of(uint32_t item, const LinearParams& p) {
     uint32_t t, half, batch, tn, tt;
     rb_gemm_item(item, p.split, t, half);
     rb_tile_coords(t, p.tiles_n, p.tiles_t, GROUP, batch, tn, tt);
-    const uint32_t tokens = half == 2 ? PAIR_TOKENS : PAIR_TOKENS / 2;
-    return {tn * 2 * ROWS, tt * PAIR_TOKENS + (half == 2 ? 0 : half * tokens), tokens};
+    const uint32_t tokens = half == 2 ? p.tokens : p.tokens / 2;
+    return {tn * 2 * ROWS, tt * p.tokens + (half == 2 ? 0 : half * tokens), tokens};
 }
 
+template <typename Out>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 linear_i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_xh, const LinearParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -256,7 +356,7 @@ linear_i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             for (uint32_t t = pair; ok && t < p.items; t += pairs) {
                 const Item it = item_of(t, p);
                 const uint32_t rows = it.tokens / 2;
-                const CUtensorMap* mx = it.tokens == PAIR_TOKENS ? &map_x : &map_xh;
+                const CUtensorMap* mx = it.tokens == p.tokens ? &map_x : &map_xh;
                 for (uint32_t kb = 0; kb < p.num_kb; ++kb) {
                     if (!(ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_word))) break;
                     uint8_t* sa = smem + stage * PAIR_STAGE_BYTES;
@@ -275,7 +375,7 @@ linear_i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             uint32_t stage = 0, phase = 0, iter = 0;
             for (uint32_t t = pair; ok && t < p.items; t += pairs, ++iter) {
                 const uint32_t acc = iter & 1, acc_phase = (iter >> 1) & 1;
-                const uint32_t idesc = t < p.split ? idesc_i8(2 * ROWS, PAIR_TOKENS) : idesc_i8(2 * ROWS, PAIR_TOKENS / 2);
+                const uint32_t idesc = idesc_i8(2 * ROWS, t < p.split ? p.tokens : p.tokens / 2);
                 if (!(ok = mbar_wait(&tmem_empty[acc], acc_phase ^ 1, abort_word))) break;
                 tc_fence_after();
                 const uint32_t tmem_d = tmem_base + acc * PAIR_TOKENS;
@@ -312,10 +412,7 @@ linear_i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                 uint32_t r[32];
                 tmem_ld_32x32(tmem_base + acc * PAIR_TOKENS + ((quarter * 32) << 16) + c, r);
                 tmem_wait_ld();
-                if (col < p.n) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) if (it.token0 + c + j < p.m) put(p, it.token0 + c + j, col, (int32_t)r[j], sx[c + j], sw, bias);
-                }
+                put<Out, 32>(p, it.token0 + c, col, r, sx + c, sw, bias, p.m - it.token0 - c);
             }
             tc_fence_before();
             mbar_arrive_cluster(mapa_shared(smem_u32(&tmem_empty[acc]), 0));   // 128 arrivals from each CTA of the pair
@@ -340,11 +437,12 @@ bool byte_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t k, uin
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int TOKENS>
+template <typename Out, int TOKENS>
 int32_t launch_few(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, uint32_t k, uint32_t parts) {
+    auto* kernel = linear_i8_few_kernel<Out, TOKENS>;
     static std::once_flag once;
     static cudaError_t configured = cudaSuccess;
-    std::call_once(once, [] { configured = cudaFuncSetAttribute(linear_i8_few_kernel<TOKENS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<TOKENS>::SMEM_BYTES); });
+    std::call_once(once, [kernel] { configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<TOKENS>::SMEM_BYTES); });
     if (configured != cudaSuccess) return rb::fail(RB_STATUS, "cudaFuncSetAttribute(8-bit linear) failed with CUDA status %d (%s)", (int)configured, cudaGetErrorString(configured));
     CUtensorMap mw, mx;
     if (!byte_map(&mw, w, p.n, k, ROWS) || !byte_map(&mx, x, p.m, k, TOKENS)) return rb::fail(RB_STATUS, "cuTensorMapEncodeTiled failed for the 8-bit linear (m=%u n=%u k=%u)", p.m, p.n, k);
@@ -354,36 +452,91 @@ int32_t launch_few(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, u
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension; attr.val.clusterDim.x = parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
     cfg.attrs = &attr; cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, linear_i8_few_kernel<TOKENS>, mw, mx, p);     // a failure is what after_launch reports
+    cudaLaunchKernelEx(&cfg, kernel, mw, mx, p);     // a failure is what after_launch reports
     return rb::after_launch(ctx, "8-bit linear (few tokens)");
 }
 
-int32_t launch_pair(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, uint32_t k) {
+// CTA pairs that can be resident at once (not every SM can be paired), capped by the context's SM limit; 0 after a failure.
+uint32_t resident_pairs(rb_ctx* ctx) {
     static std::once_flag once;
-    static cudaError_t configured = cudaSuccess;
     static int clusters = 0;
     const int sms = ctx->sm_count;
     std::call_once(once, [sms] {
-        configured = cudaFuncSetAttribute(linear_i8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM_BYTES);
+        for (auto* kernel : {linear_i8_pair_kernel<float>, linear_i8_pair_kernel<bf>, linear_i8_pair_kernel<__half>})
+            if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM_BYTES) != cudaSuccess) return;
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(2 * (unsigned)sms); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = PAIR_SMEM_BYTES;
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeClusterDimension; attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
         cfg.attrs = &attr; cfg.numAttrs = 1;
-        if (configured == cudaSuccess) configured = cudaOccupancyMaxActiveClusters(&clusters, linear_i8_pair_kernel, &cfg);
+        if (cudaOccupancyMaxActiveClusters(&clusters, linear_i8_pair_kernel<bf>, &cfg) != cudaSuccess) clusters = 0;
     });
-    if (configured != cudaSuccess || clusters < 1) return rb::fail(RB_STATUS, "configuring the 8-bit linear failed with CUDA status %d (%s)", (int)configured, cudaGetErrorString(configured));
     uint32_t pairs = (uint32_t)clusters;
-    if (ctx->sm_limit > 0 && (uint32_t)ctx->sm_limit / 2 < pairs) pairs = (uint32_t)ctx->sm_limit / 2;
-    if (pairs == 0) pairs = 1;
-    p.tiles_n = (p.n + 2 * ROWS - 1) / (2 * ROWS); p.tiles_t = (p.m + PAIR_TOKENS - 1) / PAIR_TOKENS;
-    rb_gemm_plan(p.tiles_n * p.tiles_t, pairs, true, p.split, p.items);
+    if (ctx->sm_limit > 0 && (uint32_t)ctx->sm_limit / 2 < pairs) pairs = (uint32_t)ctx->sm_limit < 2 ? 1 : (uint32_t)ctx->sm_limit / 2;
+    return pairs;
+}
+
+template <typename Out>
+int32_t launch_pair(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, uint32_t k, uint32_t pairs, uint32_t tokens) {
+    p.tokens = tokens;
+    p.tiles_n = (p.n + 2 * ROWS - 1) / (2 * ROWS); p.tiles_t = (p.m + tokens - 1) / tokens;
+    rb_gemm_plan(p.tiles_n * p.tiles_t, pairs, tokens % 64 == 0, p.split, p.items);
     if (p.items < pairs) pairs = p.items;
     CUtensorMap mw, mx, mxh;
-    if (!byte_map(&mw, w, p.n, k, ROWS) || !byte_map(&mx, x, p.m, k, PAIR_TOKENS / 2) || !byte_map(&mxh, x, p.m, k, PAIR_TOKENS / 4))
+    if (!byte_map(&mw, w, p.n, k, ROWS) || !byte_map(&mx, x, p.m, k, tokens / 2) || !byte_map(&mxh, x, p.m, k, tokens / 4))
         return rb::fail(RB_STATUS, "cuTensorMapEncodeTiled failed for the 8-bit linear (m=%u n=%u k=%u)", p.m, p.n, k);
-    linear_i8_pair_kernel<<<2 * pairs, THREADS, PAIR_SMEM_BYTES, ctx->stream>>>(mw, mx, mxh, p);
+    linear_i8_pair_kernel<Out><<<2 * pairs, THREADS, PAIR_SMEM_BYTES, ctx->stream>>>(mw, mx, mxh, p);
     return rb::after_launch(ctx, "8-bit linear (CTA pairs)");
+}
+
+template <typename Out>
+int32_t launch_rows(rb_ctx* ctx, const LinearParams& p, const void* w, const void* x, uint32_t k) {
+    const int8_t* xp = static_cast<const int8_t*>(x); const int8_t* wp = static_cast<const int8_t*>(w);
+    // More rows a warp (R) mean fewer loads of x and fewer warps.  us for n x k and m tokens at R = 1 / 2 / 4: 1024 x 4096, 1: 3.0 / 3.7 / 5.3;
+    // 6144 x 4096, 1: 6.8 / 5.9 / 7.2; 6144 x 4096, 4: - / 9.1 / 6.9; 4096 x 4096, 4: 6.6 / 6.2 / 6.1.
+    const uint32_t sms = (uint32_t)ctx->sm_count;
+#define RB_ROWS(M, R) linear_i8_row_kernel<Out, M, R><<<(p.n + 4 * R - 1) / (4 * R), 128, 0, ctx->stream>>>(xp, wp, p, k)
+    if (p.m == 1) { if (p.n <= 32 * sms) RB_ROWS(1, 1); else RB_ROWS(1, 2); }
+    else if (p.m == 2) { if (p.n <= 16 * sms) RB_ROWS(2, 1); else RB_ROWS(2, 2); }
+    else { if (p.n <= 32 * sms) RB_ROWS(4, 2); else RB_ROWS(4, 4); }
+#undef RB_ROWS
+    return rb::after_launch(ctx, "8-bit linear (rows)");
+}
+
+// tokens: width of a tile; parts: CTAs that share K.  parts 0: CTA pairs; tokens 0: rows.
+struct Plan { uint32_t tokens, parts; };
+
+template <typename Out>
+int32_t launch(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, uint32_t k, const Plan& plan, uint32_t pairs) {
+    if (plan.tokens == 0) return launch_rows<Out>(ctx, p, w, x, k);
+    if (plan.parts == 0) return launch_pair<Out>(ctx, p, w, x, k, pairs, plan.tokens);
+    switch (plan.tokens) {
+        case 16: return launch_few<Out, 16>(ctx, p, w, x, k, plan.parts);
+        case 32: return launch_few<Out, 32>(ctx, p, w, x, k, plan.parts);
+        case 64: return launch_few<Out, 64>(ctx, p, w, x, k, plan.parts);
+        default: return launch_few<Out, 128>(ctx, p, w, x, k, plan.parts);
+    }
+}
+
+// Which kernel, by the sizes alone.  Figures: us on one B200, weights from DRAM, BF16 result.
+Plan plan_of(const LinearParams& p, uint32_t sms, uint32_t pairs) {
+    auto tiles = [&](uint32_t rows, uint32_t tokens) { return (uint64_t)((p.n + rows - 1) / rows) * ((p.m + tokens - 1) / tokens); };
+    auto share = [&](uint64_t ctas, uint64_t t) { uint64_t s = ctas / t; s = s < 8 ? s : 8; s = s < p.num_kb ? s : p.num_kb; return (uint32_t)(s ? s : 1); };
+    // One or two tokens, and up to four over short rows: no tensor core, no set-up (6144 x 4096: 5.9 / 6.7 / 6.9 for 1 / 2 / 4 tokens against
+    // 8.3; 4096 x 14336: 10.9 / 12.1 / 14.4 against 13.6).
+    if (p.m <= 2 || (p.m <= 4 && p.num_kb < 96)) return {0, 0};
+    // Up to 32 tokens the weights' bytes are everything: one CTA per SM streams them (4096 x 4096, 17 tokens: 7.9 with 4 parts, 9.3 with 2,
+    // 8.5 with 8; 14336 x 4096: 14.1 unsplit, 15.5 with 2).
+    if (p.m <= 32) { const uint32_t t = p.m <= 16 ? 16 : 32; return {t, share(sms, tiles(ROWS, t))}; }
+    // Up to 64 the products and the join weigh more, and two CTAs an SM hide them (6144 x 4096, 64 tokens: 10.9 with 4 parts, 12.0 with 3).
+    if (p.m <= 64) return {64, share(sms * 4 / 3, tiles(ROWS, 64))};
+    // Few tiles: K split four ways or more beats pairs, which cannot split it (4096 x 14336, 128 tokens: 17.7 against 26; 4096 x 4096: 10.8
+    // both), above 128 tokens only for long K (256 tokens, K 14336: 21.8 against 26.3; K 4096: 13.2 against 11.4).
+    const uint32_t few = p.m <= 128 ? 64 : 128, parts = share(2 * sms, tiles(ROWS, few));
+    if (p.m <= 256 && parts >= 4 && (p.m <= 128 || p.num_kb >= 64)) return {few, parts};
+    // Pairs: 256 tokens a tile read the least from L2 and draw the least power (4096 x 14336 x 4096 sustained: 175, 128 tokens: 214);
+    // narrower ones where those would leave half of the pairs idle.
+    return {tiles(2 * ROWS, 256) * 2 <= pairs ? 128u : 256u, 0};
 }
 
 }  // namespace
@@ -415,24 +568,14 @@ int32_t rb_linear_i8(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* x_scales,
     DeviceGuard device(ctx);
     LinearParams p{};
     p.m = (uint32_t)m; p.n = (uint32_t)n; p.num_kb = (uint32_t)((k + BK - 1) / BK);
-    p.out = y->dtype == RB_F32 ? 1u : (y->dtype == RB_F16 ? 2u : 0u);
     p.sx = (const float*)psx; p.sw = (const float*)psw; p.bias = (const float*)pb; p.y = py;
     RB_TRY(kernel_status_word(ctx, &p.status));
-    uint32_t tokens = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
-    const uint32_t tiles = ((uint32_t)n + ROWS - 1) / ROWS * (((uint32_t)m + tokens - 1) / tokens);
-    uint32_t parts = (uint32_t)ctx->sm_count / tiles;
-    if (parts > 8) parts = 8;
-    if (parts > p.num_kb) parts = p.num_kb;
-    if (parts < 1) parts = 1;
-    bool pair = m > 512;
-    if (pair) return launch_pair(ctx, p, pw, px, (uint32_t)k);
-    switch (tokens) {
-        case 16: return launch_few<16>(ctx, p, pw, px, (uint32_t)k, parts);
-        case 32: return launch_few<32>(ctx, p, pw, px, (uint32_t)k, parts);
-        case 64: return launch_few<64>(ctx, p, pw, px, (uint32_t)k, parts);
-        case 128: return launch_few<128>(ctx, p, pw, px, (uint32_t)k, parts);
-        default: return launch_few<256>(ctx, p, pw, px, (uint32_t)k, parts);
-    }
+    const uint32_t pairs = resident_pairs(ctx);
+    if (pairs == 0) return fail(RB_STATUS, "%s: configuring the kernel failed", what);
+    const Plan plan = plan_of(p, (uint32_t)ctx->sm_count, pairs);
+    if (y->dtype == RB_F32) return launch<float>(ctx, p, pw, px, (uint32_t)k, plan, pairs);
+    if (y->dtype == RB_BF16) return launch<bf>(ctx, p, pw, px, (uint32_t)k, plan, pairs);
+    return launch<__half>(ctx, p, pw, px, (uint32_t)k, plan, pairs);
 }
 
 }  // extern "C"

@@ -399,7 +399,7 @@ __device__ __forceinline__ uint64_t divide(uint64_t n, const Divisor& v) { retur
 // y = q * scale on flat vectors of 16 bytes of y (q and y are contiguous, so they stay aligned whatever the width); the row of a
 // vector's first element comes from one division, a row's end inside the vector steps to the next scale.
 template <typename T, typename Index>
-__global__ void __launch_bounds__(256) dequant_kernel(const int8_t* q, const float* scales, T* y, uint64_t total, uint32_t width, const Divisor by_width) {
+__global__ void __launch_bounds__(256, 8) dequant_kernel(const int8_t* q, const float* scales, T* y, uint64_t total, uint32_t width, const Divisor by_width) {
     constexpr int PER = 16 / sizeof(T), UNROLL = 32 / PER;         // 32 elements a thread
     typedef Pack<int8_t, PER> Bytes;
     const Index vectors = (Index)(total / PER), base = (Index)blockIdx.x * 256 * UNROLL + threadIdx.x;
@@ -430,7 +430,9 @@ __global__ void __launch_bounds__(256) dequant_kernel(const int8_t* q, const flo
 #pragma unroll
         for (int j = 0; j < PER; j += 2) add2(f[j], f[j + 1], -8388736.0f, -8388736.0f);
         times<PER>(f, by);
-        reinterpret_cast<Pack<T, PER>*>(y)[v] = narrow<T, PER>(f);
+        const Pack<T, PER> o = narrow<T, PER>(f);
+        uint4 t; memcpy(&t, &o, 16);
+        __stcs(reinterpret_cast<uint4*>(y) + v, t);
     }
     const uint64_t tail = (uint64_t)vectors * PER + threadIdx.x;
     if (blockIdx.x == 0 && threadIdx.x < PER && tail < total) y[tail] = from_f32<T>(__fmul_rn((float)q[tail], scales[tail / width]));
