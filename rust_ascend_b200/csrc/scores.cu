@@ -1,17 +1,26 @@
 // Scores of single tokens from a row of logits: log probability of a given id, log-sum-exp, entropy and the largest alternatives, and
 // the gradient of the first two with respect to the logits.
 //
-// With z = scale * x and M = max x every row needs S = sum 2^d and T = sum 2^d d over d = (x - M) scale log2(e):
-//     lse = scale M + ln S,   log p = scale (x - M) - ln S,   H = ln S - ln2 T / S.
-// One pass holds them against a running maximum: when a chunk raises it, S and T are moved to the new one,
-//     f = 2^((m - m') scale log2(e)),   T <- f (T + S (m - m') scale log2(e)),   S <- f S.
-// d is held at -1000 and above (2^-1000 is 0 in FP32), which makes a logit of -inf, and a thread that has seen nothing else, count as
-// probability 0 without a special case; maxima are taken so that a NaN stays.
+// In units of log 2, with c = scale log2(e) and a reference m (the largest c x, rounded), every row needs S = sum 2^d and T = sum 2^d d
+// over d = c x - m:
+//     lse = ln2 (m + log2 S),   log p = ln2 (c x - m - log2 S),   H = ln2 (log2 S - T / S).
+// d is one fused product, and m's own rounding cancels in log p.  One pass holds S and T against a running reference: when a chunk
+// raises it, they are moved to the new one, with f = 2^(m - m'):   T <- f (T + S (m - m')),   S <- f S.
+// Logits below `low` (masks: -inf, the type's lowest value) are lifted to it, from where 2^d is 0, and the reference starts at half
+// of it; a row that never rises above that start, or holds a NaN or an infinity, is done again by careful_row.
 //
-// HBM-bound: the row is read once.  The top_k largest need no second pass over it either.  A row is split into the slices of the
-// block's threads; the k-th largest slice maximum is a lower bound of the k-th largest element, so every element of the answer
-// lies in a slice whose maximum reaches that bound (about k of them), and only those are read again (they hit L2).
+// Bounds: DRAM (the row is read once), then the exponential unit (one 2^d an element, 16 a clock and SM) and the issue slots: about
+// five instructions an element, from packed maxima, products and sums.
+//
+// The top_k largest need no second pass over the row either.  A row is split into the slices of the block's threads; the k-th largest
+// slice maximum is a lower bound of the k-th largest element, so every element of the answer lies in a slice whose maximum reaches
+// that bound (about k of them).  Threads note the maxima of up to 16 chunks of their slice, and only the chunks that reach the bound
+// are read again (they hit L2).  (The least over the warps of each warp's k/8-th largest slice maximum is a cheaper bound, but lets
+// several times as many elements through: slower at every k above 5.  Asking L2 for the next rounds ahead of the loads: slower.)
 #include "common.cuh"
+
+#include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -20,13 +29,18 @@ using bf = __nv_bfloat16;
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int CANDIDATES = 1024;      // elements at or above the bound that a block can hold; more (ties, hostile rows) take the exact search
-constexpr int UNROLL = 4;             // 16-byte vectors a thread has in flight
+constexpr int UNROLL = 4;             // 16-byte vectors a thread of the gradient has in flight
+constexpr int CHUNKS = 16;            // parts of a thread's slice whose maxima are kept
+constexpr int AGAIN = 512;            // chunks that may be read again before a row takes the exact search
 
 template <typename T> struct Traits;
-// KEY_SHIFT: low bits of the FP32 pattern that a value of the storage type never uses
-template <> struct Traits<float> { static constexpr int PER = 4, KEY_SHIFT = 0; };
-template <> struct Traits<bf> { static constexpr int PER = 8, KEY_SHIFT = 16; };
-template <> struct Traits<__half> { static constexpr int PER = 8, KEY_SHIFT = 13; };
+// BOUND_BITS: leading bits of an order key that the bound of the top list is made from: all that a 16-bit value has; for FP32 a
+// slightly lower bound lets hardly more candidates through and takes fewer steps.
+// LOG_ROUND: log2 of the 16-byte vectors that a thread has in flight (2048 rows of 32000 FP32: 44.2 us at eight, 47.7 at four; 2048 of
+// 128000 BF16, which needs more registers a vector: 95 and 90).
+template <> struct Traits<float> { static constexpr int PER = 4, BOUND_BITS = 24, LOG_ROUND = 3; };
+template <> struct Traits<bf> { static constexpr int PER = 8, BOUND_BITS = 16, LOG_ROUND = 2; };
+template <> struct Traits<__half> { static constexpr int PER = 8, BOUND_BITS = 19, LOG_ROUND = 2; };
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(bf v) { return __bfloat162float(v); }
@@ -41,48 +55,58 @@ __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32
 __device__ __forceinline__ float max_nan(float a, float b) { float y; asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b)); return y; }
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr float LEAST = -1000.0f;
+constexpr float LEAST = -1000.0f;       // 2^-1000 is 0
 
 // Integer that orders values as the top list does: larger value, larger key; both zeros alike; every NaN on top.
-template <typename T>
 __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
-    const uint32_t k = x != x ? 0xffffffffu : ((u & 0x80000000u) ? ~u : u | 0x80000000u);
-    return k >> Traits<T>::KEY_SHIFT;
+    return x != x ? 0xffffffffu : ((u & 0x80000000u) ? ~u : u | 0x80000000u);
 }
 
+typedef unsigned long long Entry;         // order key above, complement of the index below: larger is earlier in the top list, no two are equal
+__device__ __forceinline__ Entry entry_of(uint32_t key, uint32_t at) { return (Entry)key << 32 | (uint32_t)~at; }
+__device__ __forceinline__ uint32_t index_of(Entry e) { return ~(uint32_t)e; }
+__device__ __forceinline__ float value_of(Entry e) {      // order_key the other way round
+    const uint32_t k = (uint32_t)(e >> 32);
+    return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+
+// Two FP32 operations in one instruction, each rounded as the single one is.
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(a), "+f"(b) : "f"(x), "f"(y));
+}
+__device__ __forceinline__ void fma2(float& c, float& d, float a, float b, float x, float y) {      // (c, d) += (a x, b y)
+    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 r, {%0, %1};\n\tfma.rn.f32x2 r, p, q, r;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "+f"(c), "+f"(d) : "f"(a), "f"(b), "f"(x), "f"(y));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+
+// S and T against the reference m (log2 units); t is always kept as the sum over d <= 0.
 struct Stats { float m, s, t; };
 
-// (m, s, t) of two disjoint sets of elements, joined.
-__device__ __forceinline__ Stats join(const Stats& a, const Stats& b, float c2) {
-    const float m = max_nan(a.m, b.m);
-    const float da = fmaxf((a.m - m) * c2, LEAST), db = fmaxf((b.m - m) * c2, LEAST);
-    const float fa = ex2(da), fb = ex2(db);
-    return {m, fa * a.s + fb * b.s, fa * (a.t + a.s * da) + fb * (b.t + b.s * db)};
+__device__ __forceinline__ void move_to(Stats& a, float m) {
+    const float d = fmaxf(a.m - m, LEAST), f = ex2(d);
+    a.t = f * (a.t + a.s * d); a.s *= f; a.m = m;
 }
-
-template <int N>
-__device__ __forceinline__ void take(Stats& st, const float (&x)[N], float c2) {
-    float top = x[0];
-#pragma unroll
-    for (int j = 1; j < N; ++j) top = max_nan(top, x[j]);
-    top = max_nan(top, st.m);
-    if (!(top == st.m)) {
-        const float d = fmaxf((st.m - top) * c2, LEAST), f = ex2(d);
-        st.t = f * (st.t + st.s * d); st.s *= f; st.m = top;
-    }
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const float d = fmaxf((x[j] - st.m) * c2, LEAST), e = ex2(d);
-        st.s += e;
-        st.t = fmaf(e, d, st.t);
-    }
+// Two disjoint sets of elements, joined.
+__device__ __forceinline__ Stats join(Stats a, Stats b) {
+    const float m = max_nan(a.m, b.m);
+    move_to(a, m); move_to(b, m);
+    return {m, a.s + b.s, a.t + b.t};
+}
+// Over the lanes of a warp whose numbers differ below `span`.
+__device__ __forceinline__ Stats join_lanes(Stats st, int span) {
+#pragma unroll 1
+    for (int d = span >> 1; d > 0; d >>= 1)
+        st = join(st, {__shfl_xor_sync(0xffffffffu, st.m, d), __shfl_xor_sync(0xffffffffu, st.s, d), __shfl_xor_sync(0xffffffffu, st.t, d)});
+    return st;
 }
 
 struct ScoreArgs {
     const void* logits; uint64_t ld;
     const void* ids; uint32_t wide_ids; int64_t ignore;
-    float scale;
+    float scale, c, low, start;       // c = scale log2(e); logits below `low` count as masked; the reference starts at `start` = c low / 2
+    uint32_t careful;                 // the scale is so far from one that careful_row has to do every row
     float* log_probs; float* lse; float* entropy; float* top_values; int32_t* top_ids;
     uint32_t k, vocab; uint64_t rows;
     int* bad;                         // set when an id is outside the vocabulary; may be null
@@ -99,6 +123,76 @@ template <typename T> struct RowView {
     __device__ __forceinline__ const Vec<T>* vec() const { return reinterpret_cast<const Vec<T>*>(p + head); }
 };
 
+template <typename T> __device__ __forceinline__ Vec<T> filled(float v) {
+    Vec<T> x;
+#pragma unroll
+    for (int j = 0; j < Traits<T>::PER; ++j) from_f32(v, x.v[j]);
+    return x;
+}
+
+// Largest element of U vectors, in the storage type where it has a packed maximum; a NaN stays.
+template <typename T, int U>
+__device__ __forceinline__ float largest(const Vec<T> (&x)[U]) {
+    if constexpr (sizeof(T) == 4) {
+        float top = x[0].v[0];
+#pragma unroll
+        for (int u = 0; u < U; ++u) { top = max3(top, x[u].v[0], x[u].v[1]); top = max3(top, x[u].v[2], x[u].v[3]); }
+        return top;
+    } else {
+        typedef typename std::conditional<std::is_same<T, bf>::value, __nv_bfloat162, __half2>::type T2;
+        T2 top = *reinterpret_cast<const T2*>(&x[0].v[0]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) top = __hmax2_nan(top, *reinterpret_cast<const T2*>(&x[u].v[j]));
+        return max_nan(to_f32(top.x), to_f32(top.y));
+    }
+}
+// Two neighbouring elements, lifted to `low` (NaN too: the reference has it), as FP32.
+template <typename T>
+__device__ __forceinline__ void lifted(const T* p, float low, float& a, float& b) {
+    if constexpr (sizeof(T) == 4) { a = fmaxf(p[0], low); b = fmaxf(p[1], low); }
+    else if constexpr (std::is_same<T, bf>::value) {
+        const __nv_bfloat162 x = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(p), __float2bfloat162_rn(low));
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(&x);
+        a = __uint_as_float(w << 16); b = __uint_as_float(w & 0xffff0000u);
+    } else {
+        const float2 f = __half22float2(__hmax2(*reinterpret_cast<const __half2*>(p), __float2half2_rn(low)));
+        a = f.x; b = f.y;
+    }
+}
+// Adds U vectors to a thread's S and T (as two sums each) and keeps its largest element.
+struct Running { float m, s0, s1, t0, t1, most; };
+template <typename T, int U>
+__device__ __forceinline__ float take(Running& r, const Vec<T> (&x)[U], const ScoreArgs& a) {
+    const float top = largest<T, U>(x);
+    r.most = max_nan(r.most, top);
+    const float m = max_nan(r.m, top * a.c);
+    if (!(m == r.m)) {
+        Stats st{r.m, r.s0 + r.s1, r.t0 + r.t1};
+        move_to(st, m);
+        r.m = m; r.s0 = st.s; r.s1 = 0.f; r.t0 = st.t; r.t1 = 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < Traits<T>::PER; j += 2) {
+            float xa, xb, da = -r.m, db = -r.m;
+            lifted<T>(&x[u].v[j], a.low, xa, xb);
+            fma2(da, db, xa, xb, a.c, a.c);
+            const float ea = ex2(da), eb = ex2(db);
+            add2(r.s0, r.s1, ea, eb);
+            fma2(r.t0, r.t1, ea, eb, da, db);
+        }
+    return top;
+}
+
+__device__ __forceinline__ Entry ld_cluster_u64(const void* at, uint32_t rank) {
+    uint32_t a; Entry v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(rank));
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+    return v;
+}
 __device__ __forceinline__ uint32_t ld_cluster_u32(const void* at, uint32_t rank) {
     uint32_t a, v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(rank));
@@ -108,36 +202,59 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(const void* at, uint32_t rank
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
 
 struct Shared {
+    Entry entry[CANDIDATES];
+    Entry list[RB_MAX_TOP];
     Stats warp[WARPS];
+    float most[WARPS];
     Stats mine;                          // this block's part, read by the cluster's first block
-    uint32_t key[CANDIDATES], at[CANDIDATES];
-    uint32_t list_key[RB_MAX_TOP], list_at[RB_MAX_TOP];
-    uint32_t winners[THREADS];
-    uint32_t found, winner_count, list_count;
+    float chunk[CHUNKS][THREADS];        // largest element of each thread's chunks
+    uint16_t again[AGAIN];               // chunks to read again: thread + 256 * chunk
+    uint32_t found, again_count;
     uint32_t tie_warp[WARPS];
 };
 
 __device__ __forceinline__ void push(Shared& sh, uint32_t key, uint32_t at) {
     const uint32_t i = atomicAdd(&sh.found, 1u);
-    if (i < CANDIDATES) { sh.key[i] = key; sh.at[i] = at; }
+    if (i < CANDIDATES) sh.entry[i] = entry_of(key, at);
 }
 
-// Candidates -> sorted list of the first `want`.  Every (key, index) is distinct, so the number of candidates in front of one is its
-// place.
+// Candidates -> sorted list of the first `want`.  The number of candidates in front of one is its place; eight lanes count for each.
 __device__ __forceinline__ void rank_candidates(Shared& sh, uint32_t count, uint32_t want) {
-    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
-        const uint32_t key = sh.key[i], at = sh.at[i];
+    const uint32_t part = threadIdx.x & 7;
+    for (uint32_t base = 0; base < count; base += THREADS / 8) {
+        const uint32_t i = base + (threadIdx.x >> 3);
+        const Entry e = i < count ? sh.entry[i] : 0;
         uint32_t place = 0;
-        for (uint32_t j = 0; j < count; ++j) { const uint32_t kj = sh.key[j]; place += kj > key || (kj == key && sh.at[j] < at); }
-        if (place < want) { sh.list_key[place] = key; sh.list_at[place] = at; }
+#pragma unroll 4
+        for (uint32_t j = part; j < count; j += 8) place += sh.entry[j] > e;
+#pragma unroll
+        for (int d = 4; d > 0; d >>= 1) place += __shfl_xor_sync(0xffffffffu, place, d);
+        if (part == 0 && i < count && place < want) sh.list[place] = e;
+    }
+}
+// Sorted lists of k entries, one after the other in sh.entry, into one sorted list of k.  An entry's place is its place in its own list
+// and the number of larger entries in each other one, found by halving.  Empty entries (0) are behind all others and never placed.
+__device__ __forceinline__ void merge_lists(Shared& sh, uint32_t lists, uint32_t k) {
+    for (uint32_t i = threadIdx.x; i < lists * k; i += THREADS) {
+        const uint32_t own = i / k;
+        const Entry e = sh.entry[i];
+        uint32_t place = i - own * k;
+        for (uint32_t l = 0; l < lists; ++l) {
+            if (l == own) continue;
+            uint32_t lo = 0, hi = k;                      // entries [0, lo) are larger than e, entries [hi, k) are not
+            while (lo < hi) { const uint32_t mid = (lo + hi) / 2; if (sh.entry[l * k + mid] > e) lo = mid + 1; else hi = mid; }
+            place += lo;
+        }
+        if (place < k && e != 0) sh.list[place] = e;
     }
 }
 
-// The k-th largest of one key per thread, bit by bit from the top.
-template <typename T>
+// The largest bound of BITS leading bits that k of the block's keys (one per thread) reach; bit by bit from the top.
+template <int BITS>
 __device__ __forceinline__ uint32_t kth_of_block(uint32_t key, uint32_t k) {
     uint32_t bound = 0;
-    for (int bit = 31 - Traits<T>::KEY_SHIFT; bit >= 0; --bit) {
+#pragma unroll 1
+    for (int bit = 31; bit >= 32 - BITS; --bit) {
         const uint32_t trial = bound | (1u << bit);
         if ((uint32_t)__syncthreads_count(key >= trial) >= k) bound = trial;
     }
@@ -151,7 +268,7 @@ __device__ uint32_t count_in_block(Shared& sh, const T* row, uint32_t first, uin
     if (threadIdx.x == 0) sh.found = 0;
     __syncthreads();
     uint32_t n = 0;
-    for (uint32_t i = first + threadIdx.x; i < last; i += THREADS) { const uint32_t key = order_key<T>(to_f32(row[i])); n += key > bound || (or_equal && key == bound); }
+    for (uint32_t i = first + threadIdx.x; i < last; i += THREADS) { const uint32_t key = order_key(to_f32(row[i])); n += key > bound || (or_equal && key == bound); }
     n = __reduce_add_sync(0xffffffffu, n);
     if ((threadIdx.x & 31) == 0) atomicAdd(&sh.found, n);
     __syncthreads();
@@ -165,7 +282,7 @@ template <typename T>
 __device__ __noinline__ void exact_candidates(Shared& sh, const T* row, uint32_t first, uint32_t last, uint32_t bound, uint32_t want) {
     if (count_in_block<T>(sh, row, first, last, bound, false) > CANDIDATES) {
         bound = 0;
-        for (int bit = 31 - Traits<T>::KEY_SHIFT; bit >= 0; --bit) {
+        for (int bit = 31; bit >= 0; --bit) {
             const uint32_t trial = bound | (1u << bit);
             if (count_in_block<T>(sh, row, first, last, trial, true) >= want) bound = trial;
         }
@@ -173,12 +290,12 @@ __device__ __noinline__ void exact_candidates(Shared& sh, const T* row, uint32_t
     __syncthreads();
     if (threadIdx.x == 0) sh.found = 0;
     __syncthreads();
-    for (uint32_t i = first + threadIdx.x; i < last; i += THREADS) { const uint32_t key = order_key<T>(to_f32(row[i])); if (key > bound) push(sh, key, i); }
+    for (uint32_t i = first + threadIdx.x; i < last; i += THREADS) { const uint32_t key = order_key(to_f32(row[i])); if (key > bound) push(sh, key, i); }
     __syncthreads();
     uint32_t have = sh.found;                         // at most CANDIDATES by the search above; want - 1 at most where it tightened the bound
     for (uint32_t base = first; base < last && have < want; base += THREADS) {      // all threads see the same `have`
         const uint32_t i = base + threadIdx.x;
-        const bool tie = i < last && order_key<T>(to_f32(row[i])) == bound;
+        const bool tie = i < last && order_key(to_f32(row[i])) == bound;
         const uint32_t ballot = __ballot_sync(0xffffffffu, tie);
         __syncthreads();                              // the counts of the round before have been read
         if ((threadIdx.x & 31) == 0) sh.tie_warp[threadIdx.x >> 5] = __popc(ballot);
@@ -187,7 +304,7 @@ __device__ __noinline__ void exact_candidates(Shared& sh, const T* row, uint32_t
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) { if (w < (int)(threadIdx.x >> 5)) before += sh.tie_warp[w]; total += sh.tie_warp[w]; }
         const uint32_t place = have + before + __popc(ballot & ((1u << (threadIdx.x & 31)) - 1));
-        if (tie && place < want) { sh.key[place] = bound; sh.at[place] = i; }
+        if (tie && place < want) sh.entry[place] = entry_of(bound, i);
         have += total;
     }
     __syncthreads();
@@ -195,14 +312,41 @@ __device__ __noinline__ void exact_candidates(Shared& sh, const T* row, uint32_t
     __syncthreads();
 }
 
+// A whole row by one block, for the rows that the fast form does not answer: nothing but masks, infinities, NaN, scales far from one.
+// The exponent is (x - M) c with M the largest element itself, held at -1000 and above, where a logit of -inf then counts as 0.
+// m of the result is M, not its product with c.
+template <typename T>
+__device__ __noinline__ Stats careful_row(Shared& sh, const T* row, uint32_t vocab, float c) {
+    float most = -INFINITY;
+    for (uint32_t i = threadIdx.x; i < vocab; i += THREADS) most = max_nan(most, to_f32(row[i]));
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.most[threadIdx.x >> 5] = most;
+    __syncthreads();
+    for (int w = 0; w < WARPS; ++w) most = max_nan(most, sh.most[w]);
+    float s = 0.f, t = 0.f;
+    for (uint32_t i = threadIdx.x; i < vocab; i += THREADS) {
+        const float d = fmaxf((to_f32(row[i]) - most) * c, LEAST), e = ex2(d);
+        s += e; t = fmaf(e, d, t);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, d); t += __shfl_xor_sync(0xffffffffu, t, d); }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = {most, s, t};
+    __syncthreads();
+    s = 0.f; t = 0.f;
+    for (int w = 0; w < WARPS; ++w) { s += sh.warp[w].s; t += sh.warp[w].t; }
+    return {most, s, t};
+}
+
 // One row per cluster of `parts` blocks (one block where parts is 1), rows in a grid-stride loop.
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArgs a, const uint32_t parts) {
-    constexpr int PER = Traits<T>::PER;
+    constexpr int PER = Traits<T>::PER, ROUND = 1 << Traits<T>::LOG_ROUND;
     __shared__ Shared sh;
     const uint32_t tid = threadIdx.x, lane = tid & 31, rank = parts > 1 ? blockIdx.x % parts : 0;
     const uint64_t clusters = gridDim.x / parts;
-    const float c2 = a.scale * LOG2E;
     for (uint64_t r = blockIdx.x / parts; r < a.rows; r += clusters) {
         const T* row = static_cast<const T*>(a.logits) + r * a.ld;
         const RowView<T> view(row, a.vocab);
@@ -220,89 +364,118 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
             if (id != a.ignore && id >= 0 && id < (int64_t)a.vocab) chosen = to_f32(row[id]);
         }
 
-        Stats st{-INFINITY, 0.f, 0.f};
+        Running run{a.start, 0.f, 0.f, 0.f, 0.f, -INFINITY};
         const Vec<T>* vec = view.vec();
-        for (uint32_t v = v0 + tid; v < v1; v += THREADS * UNROLL) {
-            Vec<T> got[UNROLL];
+        // a chunk is 2^chunk_shift rounds of ROUND vectors, so that CHUNKS of them cover the slice
+        const uint32_t rounds = (v1 - v0 + THREADS * ROUND - 1) / (THREADS * ROUND);
+        uint32_t chunk_shift = 0;
+        while ((CHUNKS << chunk_shift) < (int)rounds) ++chunk_shift;
+        uint32_t v = v0 + tid, round = 0;
+        float chunk_top = -INFINITY;
+        auto note = [&](float top) {
+            chunk_top = max_nan(chunk_top, top);
+            if (a.k) sh.chunk[round >> chunk_shift][tid] = chunk_top;
+            if ((++round & ((1u << chunk_shift) - 1)) == 0) chunk_top = -INFINITY;
+        };
+        for (; v + (ROUND - 1) * THREADS < v1; v += THREADS * ROUND) {
+            Vec<T> got[ROUND];
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) if (v + u * THREADS < v1) got[u] = vec[v + u * THREADS];
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                float x[PER];
-#pragma unroll
-                for (int j = 0; j < PER; ++j) x[j] = v + u * THREADS < v1 ? to_f32(got[u].v[j]) : -INFINITY;
-                take<PER>(st, x, c2);
-            }
+            for (int u = 0; u < ROUND; ++u) got[u] = vec[v + u * THREADS];
+            note(take<T, ROUND>(run, got, a));
         }
-        if (tid < loose) { const float x[1] = {to_f32(row[loose_at])}; take<1>(st, x, c2); }
-        const uint32_t slice_key = order_key<T>(st.m);
+        if (v < v1) {
+            Vec<T> got[ROUND];
+#pragma unroll
+            for (int u = 0; u < ROUND; ++u) got[u] = v + u * THREADS < v1 ? vec[v + u * THREADS] : filled<T>(-INFINITY);
+            note(take<T, ROUND>(run, got, a));
+        }
+        if (tid < loose) {
+            Vec<T> got[1] = {filled<T>(-INFINITY)};
+            got[0].v[0] = row[loose_at];
+            take<T, 1>(run, got, a);
+        }
+        const uint32_t slice_key = order_key(run.most);
 
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-            const Stats o{__shfl_xor_sync(0xffffffffu, st.m, d), __shfl_xor_sync(0xffffffffu, st.s, d), __shfl_xor_sync(0xffffffffu, st.t, d)};
-            st = join(st, o, c2);
-        }
+        Stats st = join_lanes({run.m, run.s0 + run.s1, run.t0 + run.t1}, 32);
         if (lane == 0) sh.warp[tid >> 5] = st;
-        if (tid == 0) { sh.found = 0; sh.winner_count = 0; }
+        if (tid == 0) { sh.found = 0; sh.again_count = 0; }
         __syncthreads();
-        st = sh.warp[0];
-#pragma unroll
-        for (int w = 1; w < WARPS; ++w) st = join(st, sh.warp[w], c2);
+        if (tid < 32) st = join_lanes(sh.warp[lane % WARPS], WARPS);
 
         uint32_t want = 0;
         if (a.k) {
             want = a.k < last - first ? a.k : last - first;
-            const uint32_t bound = kth_of_block<T>(slice_key, a.k);
-            if (slice_key >= bound) sh.winners[atomicAdd(&sh.winner_count, 1u)] = tid;
-            if (tid < loose) { const uint32_t key = order_key<T>(to_f32(row[loose_at])); if (key >= bound) push(sh, key, loose_at); }
+            const uint32_t bound = kth_of_block<Traits<T>::BOUND_BITS>(slice_key, a.k);
+            if (slice_key >= bound) {
+                const uint32_t mine = (round + (1u << chunk_shift) - 1) >> chunk_shift;
+                for (uint32_t c = 0; c < mine; ++c)
+                    if (order_key(sh.chunk[c][tid]) >= bound) { const uint32_t i = atomicAdd(&sh.again_count, 1u); if (i < AGAIN) sh.again[i] = (uint16_t)(tid | c << 8); }
+            }
+            if (tid < loose) { const uint32_t key = order_key(to_f32(row[loose_at])); if (key >= bound) push(sh, key, loose_at); }
             __syncthreads();
-            const uint32_t winners = sh.winner_count, steps = (v1 - v0 + THREADS - 1) / THREADS;
-            for (uint32_t i = tid; i < winners * steps; i += THREADS) {
-                const uint32_t v = v0 + sh.winners[i % winners] + (i / winners) * THREADS;
-                if (v < v1) {
-                    const Vec<T> got = vec[v];
+            const uint32_t again = sh.again_count;
+            if (again <= AGAIN) {
+                const uint32_t per = Traits<T>::LOG_ROUND + chunk_shift;        // log2 of a chunk's vectors
+                for (uint32_t i = tid; i < again << per; i += THREADS) {
+                    const uint32_t which = sh.again[i >> per], at = v0 + (which & 255) + ((which >> 8 << per) + (i & ((1u << per) - 1))) * THREADS;
+                    if (at < v1) {
+                        const Vec<T> got = vec[at];
+                        uint32_t hits = 0;
 #pragma unroll
-                    for (int j = 0; j < PER; ++j) { const uint32_t key = order_key<T>(to_f32(got.v[j])); if (key >= bound) push(sh, key, view.head + v * PER + j); }
+                        for (int j = 0; j < PER; ++j) hits |= (uint32_t)(order_key(to_f32(got.v[j])) >= bound) << j;
+                        if (hits) {
+                            uint32_t i = atomicAdd(&sh.found, (uint32_t)__popc(hits));
+#pragma unroll
+                            for (int j = 0; j < PER; ++j) if ((hits >> j & 1) && i++ < CANDIDATES) sh.entry[i - 1] = entry_of(order_key(to_f32(got.v[j])), view.head + at * PER + j);
+                        }
+                    }
                 }
             }
             __syncthreads();
-            if (sh.found > CANDIDATES) exact_candidates<T>(sh, row, first, last, bound, want);
+            if (again > AGAIN || sh.found > CANDIDATES) exact_candidates<T>(sh, row, first, last, bound, want);
             rank_candidates(sh, sh.found, want);
         }
         if (parts > 1) {
-            if (tid == 0) { sh.mine = st; sh.list_count = want; }
+            if (tid == 0) sh.mine = st;
+            if (tid >= want && tid < a.k) sh.list[tid] = 0;      // fewer elements than entries
             cluster_sync();
             if (rank == 0) {
-                for (uint32_t s = 1; s < parts; ++s) {
-                    const Stats o{__uint_as_float(ld_cluster_u32(&sh.mine.m, s)), __uint_as_float(ld_cluster_u32(&sh.mine.s, s)), __uint_as_float(ld_cluster_u32(&sh.mine.t, s))};
-                    st = join(st, o, c2);
+                // one part per lane of the first warp; one list entry per thread
+                if (tid < 32) {
+                    const uint32_t from = lane % parts;      // parts is 2, 4 or 8
+                    st = join_lanes({__uint_as_float(ld_cluster_u32(&sh.mine.m, from)), __uint_as_float(ld_cluster_u32(&sh.mine.s, from)),
+                                     __uint_as_float(ld_cluster_u32(&sh.mine.t, from))}, (int)parts);
                 }
                 if (a.k) {
-                    uint32_t count = 0;
-                    for (uint32_t s = 0; s < parts; ++s) {
-                        const uint32_t n = ld_cluster_u32(&sh.list_count, s);
-                        if (tid < n) { sh.key[count + tid] = ld_cluster_u32(&sh.list_key[tid], s); sh.at[count + tid] = ld_cluster_u32(&sh.list_at[tid], s); }
-                        count += n;
-                    }
+                    for (uint32_t i = tid; i < parts * a.k; i += THREADS) sh.entry[i] = ld_cluster_u64(&sh.list[i % a.k], i / a.k);
                     __syncthreads();
-                    rank_candidates(sh, count, a.k);
+                    merge_lists(sh, parts, a.k);
                 }
             }
         }
         if (rank == 0) {
-            const float logs = logf(st.s);
+            // the joined result is with the first warp; every thread learns whether it stands
+            if (tid == 0) sh.mine = st;
+            __syncthreads();
+            st = sh.mine;
+            const bool fast = !a.careful && st.m > a.start && st.m < 1e35f;
+            float reference, logs;               // log p of x is ln2 (c x - reference) - logs, or scale (x - reference) - logs
+            if (fast) { reference = st.m; logs = LN2 * log2f(st.s); }
+            else { st = careful_row<T>(sh, row, a.vocab, a.c); reference = st.m; logs = logf(st.s); }
+            const float lse = fast ? fmaf(LN2, reference, logs) : fmaf(reference, a.scale, logs);
+            auto log_p = [&](float x) {
+                if (!fast) return fmaf(x - reference, a.scale, -logs);
+                return x < a.low ? fmaf(x, a.scale, -lse) : fmaf(LN2, fmaf(x, a.c, -reference), -logs);      // c x of a mask's lowest value would overflow
+            };
             if (tid == 0) {
-                a.lse[r] = fmaf(st.m, a.scale, logs);
-                a.log_probs[r] = id == a.ignore ? 0.f : fmaf(chosen - st.m, a.scale, -logs);
+                a.lse[r] = lse;
+                a.log_probs[r] = id == a.ignore ? 0.f : log_p(chosen);
                 if (a.entropy) { const float h = logs - LN2 * (st.t / st.s); a.entropy[r] = h < 0.f ? 0.f : h; }
             }
-            if (a.k) {
-                __syncthreads();
-                if (tid < a.k) {
-                    const uint32_t at = sh.list_at[tid];
-                    a.top_ids[r * a.k + tid] = (int32_t)at;
-                    a.top_values[r * a.k + tid] = fmaf(to_f32(row[at]) - st.m, a.scale, -logs);
-                }
+            if (tid < a.k) {
+                const Entry e = sh.list[tid];
+                a.top_ids[r * a.k + tid] = (int32_t)index_of(e);
+                a.top_values[r * a.k + tid] = log_p(value_of(e));
             }
         }
         if (parts > 1) cluster_sync();       // the lists of this row have been read
@@ -378,11 +551,16 @@ bool is_float(uint32_t dtype) { return dtype == RB_F32 || dtype == RB_BF16 || dt
 
 template <typename T>
 void launch_scores(rb_ctx* ctx, const ScoreArgs& a) {
-    // A row is one block's work where the rows alone fill the GPU; fewer rows are split over clusters of up to eight blocks, as
-    // long as each thread keeps a few vectors.
-    const uint64_t slots = (uint64_t)ctx->sm_count * 4;
+    // A row is one block's work where the rows fill the GPU or are short; few long rows are split over clusters of two or four blocks.
+    // us for 4 rows at 1 / 2 / 4 / 8 blocks a row: 128000 BF16, 20 alternatives 15.4 / 12.7 / 10.8 / 11.0; 32000 BF16 8.1 / 8.9 / 9.0 / 10.0
+    // (the join of the lists costs what the split saves); for 148 rows of 128000: 22.6 / 18.4 / 27.7 / 49.
+    static std::once_flag once;
+    static int resident = 0;
+    std::call_once(once, [] { if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, token_scores_kernel<T>, THREADS, 0) != cudaSuccess || resident < 1) resident = 4; });
+    const uint64_t slots = (uint64_t)ctx->sm_count * resident, bytes = (uint64_t)a.vocab * sizeof(T);
     uint32_t parts = 1;
-    while (parts < 8 && a.rows * parts * 2 <= slots && a.vocab / Traits<T>::PER >= parts * 2 * THREADS * 2) parts *= 2;
+    if (bytes >= (a.k ? 160u : 96u) * 1024)
+        while (parts < 4 && a.rows * parts * 2 <= 3ull * ctx->sm_count) parts *= 2;
     const uint64_t clusters = a.rows < slots / parts ? a.rows : slots / parts;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(clusters * parts)); cfg.blockDim = dim3(THREADS); cfg.stream = ctx->stream;
@@ -442,7 +620,12 @@ int32_t rb_token_log_probs(rb_ctx* ctx, const rb_tensor* logits, const rb_tensor
     }
     if (rows == 0) return empty_call(ctx);
     DeviceGuard device(ctx);
-    ScoreArgs a{in.logits.ptr, in.logits.ld, in.ids, ids->dtype == RB_I64, ignore_index, scale, (float*)out[0], (float*)out[1], (float*)out[2], (float*)out[3], (int32_t*)out[4],
+    // `low`: what lies below it has probability 0 beside anything above low / 2, and c low does not overflow
+    const double c = (double)scale * 1.4426950408889634074;
+    const bool half = logits->dtype == RB_F16;
+    const double low = half ? -65504.0 : -std::fmin(1e30, 1e36 / c);
+    const bool careful = c < (half ? 0.01 : 1e-15) || c > (half ? 1e30 : 1e15);
+    ScoreArgs a{in.logits.ptr, in.logits.ld, in.ids, ids->dtype == RB_I64, ignore_index, scale, (float)c, (float)low, (float)(0.5 * low * c), careful, (float*)out[0], (float*)out[1], (float*)out[2], (float*)out[3], (int32_t*)out[4],
                 top_k, (uint32_t)in.logits.width, rows, nullptr};
     if (ctx->synchronous) {          // reports an id outside the vocabulary, as the other indexed operators do
         RB_TRY(ensure_workspace(ctx, 256));
