@@ -112,6 +112,10 @@ struct ScoreArgs {
     int* bad;                         // set when an id is outside the vocabulary; may be null
 };
 
+// Read or written once: first to leave the caches (gradient of 2048 x 128000 BF16: 156 us, with plain accesses 182).
+template <typename T> __device__ __forceinline__ Vec<T> load_streaming(const Vec<T>* p) { const uint4 t = __ldcs(reinterpret_cast<const uint4*>(p)); Vec<T> v; memcpy(&v, &t, 16); return v; }
+template <typename T> __device__ __forceinline__ void store_streaming(Vec<T>* p, const Vec<T>& v) { uint4 t; memcpy(&t, &v, 16); __stcs(reinterpret_cast<uint4*>(p), t); }
+
 // A row as aligned 16-byte vectors with up to PER - 1 elements in front and behind.
 template <typename T> struct RowView {
     const T* p; uint32_t head, vectors, vocab;
@@ -527,7 +531,7 @@ __global__ void __launch_bounds__(THREADS) token_scores_grad_kernel(const GradAr
     Vec<T>* o = reinterpret_cast<Vec<T>*>(out + view.head);
     Vec<T> got[UNROLL];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) if (first + u * THREADS < view.vectors) got[u] = in[first + u * THREADS];
+    for (int u = 0; u < UNROLL; ++u) if (first + u * THREADS < view.vectors) got[u] = load_streaming(in + first + u * THREADS);
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         const uint32_t v = first + u * THREADS;
@@ -536,7 +540,7 @@ __global__ void __launch_bounds__(THREADS) token_scores_grad_kernel(const GradAr
         Vec<T> d;
 #pragma unroll
         for (int j = 0; j < PER; ++j) from_f32(one(at + j, to_f32(got[u].v[j])), d.v[j]);
-        o[v] = d;
+        store_streaming(o + v, d);
     }
     if (seg == 0) {      // the elements around the vectors
         const uint32_t loose = a.vocab - view.vectors * PER;
