@@ -212,6 +212,31 @@ template <typename H, int VEC> struct Held {
     }
 };
 
+// What a row's values are multiplied by before they are rounded, from its largest magnitude (as bits) and, for the norm, its sum of
+// squares; `first` stores the scale.  `raise`: the values are raised by 2^96 (exactly) first, where the factor would leave FP32's range.
+struct Factor { float c; bool bad, raise; };
+template <bool NORMS>
+__device__ __forceinline__ Factor factor_of(const QuantArgs& a, uint64_t row, uint32_t bits, float sum, bool first) {
+    const bool bad = bits >= 0x7f800000u || (NORMS && sum != sum);
+    const float most = __uint_as_float(bits);
+    const float least = 1.17549435e-38f;           // 2^-126
+    const bool raise = most < 1e-16f;
+    float c = __fdiv_rn(127.0f, most);
+    // rows so small (or a norm so large) that the scale may end at 2^-126
+    const bool small = raise || (NORMS && sum > 3.4028235e38f);
+    if (first || small) {
+        const float r = NORMS ? __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)a.width), a.eps))) : 1.0f;
+        const float wanted = __fdiv_rn(__fmul_rn(r, most), 127.0f);
+        const bool tiny = wanted < least;
+        if (first) a.scales[row] = bad ? __int_as_float(0x7fc00000) : (tiny ? least : wanted);
+        if (small) {
+            c = tiny ? __fmul_rn(r, 1073741824.0f) : __fdiv_rn(127.0f, __fmul_rn(most, 7.9228163e28f));       // r 2^126, or 127 / max, over 2^96
+            if (!raise) c = __fmul_rn(c, 7.9228163e28f);
+        }
+    }
+    return {c, bad, raise};
+}
+
 // `warps` whole warps share a row: the whole block, or one warp where that is enough (a block then holds eight rows, which do not
 // wait for each other).  Everything that the threads of a row compute alike is kept to one division: the root and the scale are the
 // first thread's business.
@@ -297,24 +322,9 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
             }
             if (gridDim.x < a.rows) __syncthreads();
         }
-        const bool bad = bits >= 0x7f800000u || (NORMS && sum != sum);
-        const float a_max = __uint_as_float(bits);
-        const float least = 1.17549435e-38f;           // 2^-126
-        float c = __fdiv_rn(127.0f, a_max);
-        // Rows so small (or a norm so large) that the scale may end at 2^-126, and the factor leave FP32's range: there the values
-        // are raised by 2^96 (exactly) first.
-        const bool small = a_max < 1e-16f || (NORMS && sum > 3.4028235e38f);
-        if (tid == 0 || small) {
-            const float r = NORMS ? __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)a.width), a.eps))) : 1.0f;
-            const float wanted = __fdiv_rn(__fmul_rn(r, a_max), 127.0f);
-            const bool tiny = wanted < least, raised = a_max < 1e-16f;
-            if (tid == 0) a.scales[row] = bad ? __int_as_float(0x7fc00000) : (tiny ? least : wanted);
-            if (small) {
-                c = tiny ? __fmul_rn(r, 1073741824.0f) : __fdiv_rn(127.0f, __fmul_rn(a_max, 7.9228163e28f));       // r 2^126, or 127 / max, over 2^96
-                if (!raised) c = __fmul_rn(c, 7.9228163e28f);
-            }
-        }
-        const bool raise = a_max < 1e-16f;
+        const Factor f = factor_of<NORMS>(a, row, bits, sum, tid == 0);
+        const float c = f.c;
+        const bool bad = f.bad, raise = f.raise;
         auto finish = [&](uint32_t i, auto plain) {
             float v[VEC];
             [[maybe_unused]] float w[VEC];
@@ -330,7 +340,7 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
             }
             q[i] = to_bytes<VEC>(v, !decltype(plain)::value && bad ? 0.f : c);
         };
-        if (!bad && !small) {
+        if (!bad && !raise) {
 #pragma unroll 4
             for (uint32_t i = tid; i < vectors; i += threads) finish(i, std::true_type());
         } else {
@@ -340,6 +350,65 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
     }
 }
 
+// Plain rows that start anywhere (an odd width): vectors from the row's first 16-byte boundary on, the elements around them one by
+// one, and single bytes out.  The row lies in shared memory with its vectors aligned, so element e is at e + VEC - head, and is read
+// back by other threads than wrote it: lanes on neighbouring elements.
+template <typename T>
+__global__ void __launch_bounds__(512, 2) quant_shifted_kernel(const QuantArgs a) {
+    constexpr int VEC = 16 / sizeof(T), UNROLL = 4;
+    typedef Pack<T, VEC> In;
+    extern __shared__ __align__(16) uint8_t s_rows[];
+    __shared__ float s_most[16];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, threads = blockDim.x, tid = threadIdx.x;
+    T* held = reinterpret_cast<T*>(s_rows);
+    for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+        const uint32_t to_boundary = (uint32_t)((16u - (reinterpret_cast<uintptr_t>(x) & 15u)) & 15u) / (uint32_t)sizeof(T);
+        const uint32_t head = to_boundary < a.width ? to_boundary : a.width, vectors = (a.width - head) / VEC, shift = VEC - head;
+        const In* in = reinterpret_cast<const In*>(x + head);
+        In* out = reinterpret_cast<In*>(held) + 1;
+        float most = 0.f;
+        for (uint32_t base = tid; base < vectors; base += UNROLL * threads) {
+            In p[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) { const uint32_t i = base + u * threads; p[u] = in[i < vectors ? i : vectors - 1]; }
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const uint32_t i = base + u * threads;
+                if (i < vectors) out[i] = p[u];
+                float v[VEC];
+                widen<T, VEC>(p[u], v);
+#pragma unroll
+                for (int j = 0; j < VEC; j += 2) most = max_abs(most, v[j], v[j + 1]);
+            }
+        }
+        const uint32_t loose = a.width - vectors * VEC;
+        if (tid < loose) {
+            const uint32_t e = tid < head ? tid : vectors * VEC + tid;
+            const T v = x[e];
+            held[e + shift] = v;
+            most = max_abs(most, to_f32(v), 0.f);
+        }
+        uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+        if (lane == 0) s_most[warp] = __uint_as_float(bits);
+        __syncthreads();
+        bits = __reduce_max_sync(0xffffffffu, __float_as_uint(s_most[lane < threads / 32 ? lane : 0]));
+        const Factor f = factor_of<false>(a, row, bits, 0.f, tid == 0);
+        int8_t* q = a.q + row * a.width;
+        if (!f.bad && !f.raise) {
+#pragma unroll 4
+            for (uint32_t e = tid; e < a.width; e += threads) { const float v[1] = {to_f32(held[e + shift])}; q[e] = to_bytes<1>(v, f.c).v[0]; }
+        } else {
+            for (uint32_t e = tid; e < a.width; e += threads) {
+                const float v[1] = {f.bad ? 0.f : __fmul_rn(to_f32(held[e + shift]), 7.9228163e28f)};
+                q[e] = to_bytes<1>(v, f.bad ? 0.f : f.c).v[0];
+            }
+        }
+        if (gridDim.x < a.rows) __syncthreads();       // the row in shared memory has been read
+    }
+}
+
+constexpr uint32_t SHIFTED_VECTORS = 4;      // 1777 x 5003 FP32: 11.8 us at four vectors a thread, 12.1 at eight, 14.4 at twelve (single elements throughout: 16.0)
 constexpr uint32_t ROW_SMEM = 96 * 1024;     // shared memory a row may take: at least two rows an SM
 
 template <typename T, typename TW, int MODE, int VEC, int UNROLL>
@@ -367,6 +436,20 @@ int32_t launch(rb_ctx* ctx, QuantArgs a, const char* what) {
     return rb::after_launch(ctx, what);
 }
 
+template <typename T>
+int32_t launch_shifted(rb_ctx* ctx, const QuantArgs& a, const char* what) {
+    static std::once_flag once;
+    static cudaError_t configured = cudaSuccess;
+    std::call_once(once, [] { configured = cudaFuncSetAttribute(quant_shifted_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, ROW_SMEM); });
+    if (configured != cudaSuccess) return rb::fail(RB_STATUS, "%s: cudaFuncSetAttribute failed with CUDA status %d (%s)", what, (int)configured, cudaGetErrorString(configured));
+    const uint32_t wanted = SHIFTED_VECTORS, vectors = a.width / (16 / sizeof(T)) + 1;
+    uint32_t warps = (vectors + wanted * 32 - 1) / (wanted * 32);
+    if (warps > 16) warps = 16;
+    const uint64_t cap = 1u << 30;
+    quant_shifted_kernel<T><<<(unsigned)(a.rows < cap ? a.rows : cap), warps * 32, (a.width * sizeof(T) + 32 + 15) & ~15u, ctx->stream>>>(a);
+    return rb::after_launch(ctx, what);
+}
+
 // The widest vectors on which every row of every operand starts: 16 bytes, 8 bytes, or single elements.
 template <typename T, typename TW, int MODE>
 int32_t dispatch(rb_ctx* ctx, const QuantArgs& a, const char* what) {
@@ -379,6 +462,7 @@ int32_t dispatch(rb_ctx* ctx, const QuantArgs& a, const char* what) {
     };
     if (fits(FULL)) return launch<T, TW, MODE, FULL, MODE == ADD_NORM ? 2 : 4>(ctx, a, what);
     if (fits(HALF)) return launch<T, TW, MODE, HALF, 4>(ctx, a, what);
+    if (MODE == PLAIN && a.width >= 256 && a.width * sizeof(T) + 48 <= ROW_SMEM) return launch_shifted<T>(ctx, a, what);
     return launch<T, TW, MODE, 1, 4>(ctx, a, what);
 }
 
