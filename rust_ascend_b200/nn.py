@@ -321,6 +321,104 @@ def swiglu_frozen_bf16_fp32(input: Tensor, gate: Tensor, up: Tensor, down: Tenso
     return _wrap(c, RT.linear_frozen_bf16_fp32(c, h, down.buffer))
 
 
+# -- rows held in 8 bits, and the fixed-weight linear on them (no counterpart in the reference, whose fixed weights are BF16) ---
+@dataclass
+class QuantizedRows:
+    """Rows of 8-bit integers with one FP32 scale a row: activations [.., K], or a fixed weight [N, K] with a scale per output."""
+    values: Tensor
+    scales: Tensor
+
+    def dims(self):
+        return self.values.dims()
+
+    def dequantize(self, dtype: DType = DType.F32) -> Tensor:
+        c = _same_client(self.values, self.scales)
+        return _wrap(c, RT.dequantize_rows(c, self.values.buffer, self.scales.buffer, dtype))
+
+
+def _quantized(c, pair) -> QuantizedRows:
+    return QuantizedRows(_wrap(c, pair[0]), _wrap(c, pair[1]))
+
+
+def quantize_rows(input: Tensor) -> QuantizedRows:
+    """Rows of an FP32, BF16 or FP16 tensor, or a weight [N,K], to 8 bits."""
+    return _quantized(input.client, RT.quantize_rows(input.client, input.buffer))
+
+
+def rms_norm_quantized(input: Tensor, weight: Tensor, epsilon: float) -> QuantizedRows:
+    """rms_norm with its result in 8 bits."""
+    c = _same_client(input, weight)
+    return _quantized(c, RT.rms_norm_quant(c, input.buffer, weight.buffer, epsilon))
+
+
+def add_rms_norm_quantized(input: Tensor, delta: Tensor, weight: Tensor, epsilon: float):
+    """(input + delta rounded to the input's type, its rms_norm in 8 bits): the residual update and the norm that follows it."""
+    c = _same_client(input, delta, weight)
+    q, s, total = RT.rms_norm_quant(c, input.buffer, weight.buffer, epsilon, delta=delta.buffer)
+    return _wrap(c, total), _quantized(c, (q, s))
+
+
+def silu_mul_quantized(gate: Tensor, up: Tensor) -> QuantizedRows:
+    """silu_mul with its result in 8 bits."""
+    c = _same_client(gate, up)
+    return _quantized(c, RT.quantize_rows(c, gate.buffer, up=up.buffer))
+
+
+def linear_quantized(input: QuantizedRows, weight: QuantizedRows, bias: Tensor | None = None, dtype: DType = DType.BF16) -> Tensor:
+    """X [.., K] times a fixed W [N, K]^T, both in 8 bits, exact integer sums, result in `dtype`."""
+    c = _same_client(input.values, input.scales, weight.values, weight.scales, bias)
+    return _wrap(c, RT.linear_i8(c, input.values.buffer, input.scales.buffer, weight.values.buffer, weight.scales.buffer,
+                                 None if bias is None else bias.buffer, dtype))
+
+
+def swiglu_quantized(input: QuantizedRows, gate_up: QuantizedRows, down: QuantizedRows, dtype: DType = DType.BF16) -> Tensor:
+    """(SiLU(X Wg^T) * (X Wu^T)) Wd^T with all products on 8-bit integers.  gate_up [2 H, K] holds the gate's rows and then the up
+    projection's; its product stays in BF16 and is quantised behind SiLU * up where it lies."""
+    c = _same_client(input.values, gate_up.values, down.values)
+    rows, hidden = gate_up.dims()[0], down.dims()[1]
+    if len(input.dims()) != 2 or rows != 2 * hidden:
+        raise InvalidTensor("8-bit SwiGLU requires X[M,K], gate and up stacked as [2 H,K] and down[N,H]")
+    both = linear_quantized(input, gate_up).buffer
+    half = lambda at: TensorBuffer(both.handle, (both.shape[0], hidden), DType.BF16, (rows, 1), both.offset + at * 2, both._owner)
+    return linear_quantized(_quantized(c, RT.quantize_rows(c, half(0), up=half(hidden))), down, dtype=dtype)
+
+
+# -- scores of single tokens (the reference's loss, src/nn/causal_lm.rs:55-66, keeps only their sum) ---------------------------
+@dataclass
+class TokenScores:
+    """Of every row of logits: log probability of its token (0 where it is ignored), log-sum-exp, entropy, and the largest
+    alternatives with their log probabilities (None without alternatives)."""
+    log_probs: Tensor
+    lse: Tensor
+    entropy: Tensor
+    top_log_probs: Tensor | None
+    top_ids: Tensor | None
+    _inputs: tuple = ()
+
+    def backward(self, grad_log_probs: Tensor, grad_entropy: Tensor | None = None) -> Tensor:
+        """Gradient with respect to the logits, which must still hold what they held."""
+        logits, ids, scale, ignore = self._inputs
+        c = _same_client(logits, ids, grad_log_probs, grad_entropy)
+        return _wrap(c, RT.token_log_probs_backward(c, logits.buffer, ids.buffer, self.lse.buffer, self.entropy.buffer, grad_log_probs.buffer,
+                                                    None if grad_entropy is None else grad_entropy.buffer, scale, ignore))
+
+
+@dataclass
+class TokenScoreConfig:
+    temperature: float = 1.0
+    ignore_index: int = -100
+    alternatives: int = 0
+
+    def forward(self, logits: Tensor, ids: Tensor) -> TokenScores:
+        """Logits [.., V] in FP32, BF16 or FP16; INT32 or INT64 ids, one per row."""
+        c = _same_client(logits, ids)
+        if not (np.isfinite(self.temperature) and self.temperature > 0):
+            raise InvalidTensor("token scores need a positive, finite temperature")
+        scale = float(np.float32(1.0 / self.temperature))
+        out = RT.token_log_probs(c, logits.buffer, ids.buffer, scale, self.ignore_index, self.alternatives)
+        return TokenScores(*(None if t is None else _wrap(c, t) for t in out), _inputs=(logits, ids, scale, self.ignore_index))
+
+
 # -- attention on logical shapes of any size (src/nn/padded_attention.rs) ------------------------------------------------
 def _padded_dimensions(query, key, value, scale):
     batch, m, d = query

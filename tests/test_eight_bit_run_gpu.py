@@ -179,3 +179,36 @@ def test_steady_state_allocates_nothing(client):
     after = client.stats()
     assert after["allocations"] == before["allocations"] and after["bytes_in_use"] == before["bytes_in_use"]
     assert after["launches"] - before["launches"] == 5 * 8
+
+
+def test_nn_functions(client):
+    """The tensor-level functions: a feed-forward block, its norm, and the scores of its result."""
+    from rust_ascend_b200 import InvalidTensor, nn
+    rng = np.random.default_rng(12)
+    T = lambda a, dtype=None: nn.Tensor.from_data(client, a, dtype)
+    (xb, xv), (db, dv), (wb, wv) = (R.hold(rng.standard_normal(s), BF16) for s in ((33, 256), (33, 256), (256,)))
+    gate_up, down = ((rng.standard_normal(s) / np.sqrt(s[1])).astype(np.float32) for s in ((2 * 352, 256), (256, 352)))
+    total, q = nn.add_rms_norm_quantized(T(xb, BF16), T(db, BF16), T(wb, BF16), 1e-5)
+    alone = nn.rms_norm_quantized(total, T(wb, BF16), 1e-5)
+    assert np.array_equal(alone.values.into_data(), q.values.into_data()) and np.array_equal(alone.scales.into_data(), q.scales.into_data())
+    wg, wd = nn.quantize_rows(T(gate_up)), nn.quantize_rows(T(down))
+    y = nn.swiglu_quantized(q, wg, wd, F32)
+    h = q.dequantize().into_data().astype(np.float64)
+    both = R.hold(h @ wg.dequantize().into_data().astype(np.float64).T, BF16)[1]
+    act = nn.silu_mul_quantized(T(R.hold(both[:, :352], BF16)[0], BF16), T(R.hold(both[:, 352:], BF16)[0], BF16)).dequantize().into_data().astype(np.float64)
+    want = act @ wd.dequantize().into_data().astype(np.float64).T
+    assert np.linalg.norm(y.into_data() - want) <= 0.01 * np.linalg.norm(want)         # a BF16 rounding of `both` may fall on the other side
+    logits, ids = T((rng.standard_normal((33, 1003)) * 2).astype(np.float32)), T(rng.integers(0, 1003, 33))
+    s = nn.TokenScoreConfig(temperature=0.8, alternatives=3).forward(logits, ids)
+    w = R.scores(logits.into_data(), ids.into_data(), np.float32(1 / 0.8), -100, 3)
+    for a, b in zip((s.log_probs, s.lse, s.entropy, s.top_log_probs), w):
+        assert np.abs(a.into_data() - b).max() <= 2e-5
+    assert np.array_equal(s.top_ids.into_data(), w[4])
+    g = np.ones(33, np.float32)
+    d = s.backward(T(g), T(g)).into_data()
+    assert np.abs(d - R.scores_gradient(logits.into_data(), ids.into_data(), np.float32(1 / 0.8), -100, g, g)).max() <= 1e-5
+    assert nn.TokenScoreConfig().forward(logits, ids).top_ids is None
+    with pytest.raises(InvalidTensor, match="temperature"):
+        nn.TokenScoreConfig(temperature=0.0).forward(logits, ids)
+    with pytest.raises(InvalidTensor, match="SwiGLU"):
+        nn.swiglu_quantized(q, wd, wg)
