@@ -88,6 +88,21 @@ struct DeviceGuard {
     DeviceGuard& operator=(const DeviceGuard&) = delete;
 };
 
+// What a kernel needs before its first launch on a device (attributes, occupancy), done once per device from any thread.
+struct OncePerDevice {
+    static constexpr int DEVICES = 64;
+    std::once_flag flag[DEVICES];
+    cudaError_t status[DEVICES] = {};
+    int value[DEVICES] = {};
+    // configure(value) -> cudaError_t; the device is current
+    template <typename F> cudaError_t run(const rb_ctx* ctx, F&& configure) {
+        const int d = ctx->device;
+        if (d < 0 || d >= DEVICES) return cudaErrorInvalidDevice;
+        std::call_once(flag[d], [&] { status[d] = configure(value[d]); });
+        return status[d];
+    }
+};
+
 // Called after every kernel launch: records launch failures on the sticky list, counts the launch
 // and synchronises when the context runs in the reference's synchronous mode.
 int32_t after_launch(rb_ctx* ctx, const char* operation);

@@ -440,9 +440,8 @@ bool byte_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t k, uin
 template <typename Out, int TOKENS>
 int32_t launch_few(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, uint32_t k, uint32_t parts) {
     auto* kernel = linear_i8_few_kernel<Out, TOKENS>;
-    static std::once_flag once;
-    static cudaError_t configured = cudaSuccess;
-    std::call_once(once, [kernel] { configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<TOKENS>::SMEM_BYTES); });
+    static rb::OncePerDevice once;
+    const cudaError_t configured = once.run(ctx, [kernel](int&) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<TOKENS>::SMEM_BYTES); });
     if (configured != cudaSuccess) return rb::fail(RB_STATUS, "cudaFuncSetAttribute(8-bit linear) failed with CUDA status %d (%s)", (int)configured, cudaGetErrorString(configured));
     CUtensorMap mw, mx;
     if (!byte_map(&mw, w, p.n, k, ROWS) || !byte_map(&mx, x, p.m, k, TOKENS)) return rb::fail(RB_STATUS, "cuTensorMapEncodeTiled failed for the 8-bit linear (m=%u n=%u k=%u)", p.m, p.n, k);
@@ -458,20 +457,22 @@ int32_t launch_few(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, u
 
 // CTA pairs that can be resident at once (not every SM can be paired), capped by the context's SM limit; 0 after a failure.
 uint32_t resident_pairs(rb_ctx* ctx) {
-    static std::once_flag once;
-    static int clusters = 0;
+    static rb::OncePerDevice once;
     const int sms = ctx->sm_count;
-    std::call_once(once, [sms] {
-        for (auto* kernel : {linear_i8_pair_kernel<float>, linear_i8_pair_kernel<bf>, linear_i8_pair_kernel<__half>})
-            if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM_BYTES) != cudaSuccess) return;
+    const cudaError_t e = once.run(ctx, [sms](int& clusters) {
+        for (auto* kernel : {linear_i8_pair_kernel<float>, linear_i8_pair_kernel<bf>, linear_i8_pair_kernel<__half>}) {
+            const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM_BYTES);
+            if (set != cudaSuccess) return set;
+        }
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(2 * (unsigned)sms); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = PAIR_SMEM_BYTES;
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeClusterDimension; attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
         cfg.attrs = &attr; cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&clusters, linear_i8_pair_kernel<bf>, &cfg) != cudaSuccess) clusters = 0;
+        return cudaOccupancyMaxActiveClusters(&clusters, linear_i8_pair_kernel<bf>, &cfg);
     });
-    uint32_t pairs = (uint32_t)clusters;
+    if (e != cudaSuccess) return 0;
+    uint32_t pairs = (uint32_t)once.value[ctx->device];
     if (ctx->sm_limit > 0 && (uint32_t)ctx->sm_limit / 2 < pairs) pairs = (uint32_t)ctx->sm_limit < 2 ? 1 : (uint32_t)ctx->sm_limit / 2;
     return pairs;
 }

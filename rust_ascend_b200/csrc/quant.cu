@@ -414,9 +414,8 @@ constexpr uint32_t ROW_SMEM = 96 * 1024;     // shared memory a row may take: at
 template <typename T, typename TW, int MODE, int VEC, int UNROLL>
 int32_t launch(rb_ctx* ctx, QuantArgs a, const char* what) {
     typedef typename std::conditional<MODE == GATED, float, T>::type H;
-    static std::once_flag once;
-    static cudaError_t configured = cudaSuccess;
-    std::call_once(once, [] { configured = cudaFuncSetAttribute(quant_rows_kernel<T, TW, MODE, VEC, UNROLL>, cudaFuncAttributeMaxDynamicSharedMemorySize, ROW_SMEM); });
+    static rb::OncePerDevice once;
+    const cudaError_t configured = once.run(ctx, [](int&) { return cudaFuncSetAttribute(quant_rows_kernel<T, TW, MODE, VEC, UNROLL>, cudaFuncAttributeMaxDynamicSharedMemorySize, ROW_SMEM); });
     if (configured != cudaSuccess) return rb::fail(RB_STATUS, "%s: cudaFuncSetAttribute failed with CUDA status %d (%s)", what, (int)configured, cudaGetErrorString(configured));
     const uint32_t vectors = a.width / VEC;
     // Many rows: a few vectors a thread, so that what all threads of a row do alike weighs little and several rows share an SM (one's
@@ -438,9 +437,8 @@ int32_t launch(rb_ctx* ctx, QuantArgs a, const char* what) {
 
 template <typename T>
 int32_t launch_shifted(rb_ctx* ctx, const QuantArgs& a, const char* what) {
-    static std::once_flag once;
-    static cudaError_t configured = cudaSuccess;
-    std::call_once(once, [] { configured = cudaFuncSetAttribute(quant_shifted_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, ROW_SMEM); });
+    static rb::OncePerDevice once;
+    const cudaError_t configured = once.run(ctx, [](int&) { return cudaFuncSetAttribute(quant_shifted_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, ROW_SMEM); });
     if (configured != cudaSuccess) return rb::fail(RB_STATUS, "%s: cudaFuncSetAttribute failed with CUDA status %d (%s)", what, (int)configured, cudaGetErrorString(configured));
     const uint32_t wanted = SHIFTED_VECTORS, vectors = a.width / (16 / sizeof(T)) + 1;
     uint32_t warps = (vectors + wanted * 32 - 1) / (wanted * 32);

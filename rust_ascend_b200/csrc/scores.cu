@@ -7,7 +7,8 @@
 // d is one fused product, and m's own rounding cancels in log p.  One pass holds S and T against a running reference: when a chunk
 // raises it, they are moved to the new one, with f = 2^(m - m'):   T <- f (T + S (m - m')),   S <- f S.
 // Logits below `low` (masks: -inf, the type's lowest value) are lifted to it, from where 2^d is 0, and the reference starts at half
-// of it; a row that never rises above that start, or holds a NaN or an infinity, is done again by careful_row.
+// of it; a row that never rises above that start, holds a NaN or an infinity, or has products beyond 2^20, is done again by
+// careful_row.
 //
 // Bounds: DRAM (the row is read once), then the exponential unit (one 2^d an element, 16 a clock and SM) and the issue slots: about
 // five instructions an element, from packed maxima, products and sums.
@@ -462,7 +463,7 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
             if (tid == 0) sh.mine = st;
             __syncthreads();
             st = sh.mine;
-            const bool fast = !a.careful && st.m > a.start && st.m < 1e35f;
+            const bool fast = !a.careful && st.m > a.start && fabsf(st.m) < 1048576.0f;      // beyond 2^20 the rounding of m itself would be felt in d
             float reference, logs;               // log p of x is ln2 (c x - reference) - logs, or scale (x - reference) - logs
             if (fast) { reference = st.m; logs = LN2 * log2f(st.s); }
             else { st = careful_row<T>(sh, row, a.vocab, a.c); reference = st.m; logs = logf(st.s); }
@@ -558,9 +559,9 @@ void launch_scores(rb_ctx* ctx, const ScoreArgs& a) {
     // A row is one block's work where the rows fill the GPU or are short; few long rows are split over clusters of two or four blocks.
     // us for 4 rows at 1 / 2 / 4 / 8 blocks a row: 128000 BF16, 20 alternatives 15.4 / 12.7 / 10.8 / 11.0; 32000 BF16 8.1 / 8.9 / 9.0 / 10.0
     // (the join of the lists costs what the split saves); for 148 rows of 128000: 22.6 / 18.4 / 27.7 / 49.
-    static std::once_flag once;
-    static int resident = 0;
-    std::call_once(once, [] { if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, token_scores_kernel<T>, THREADS, 0) != cudaSuccess || resident < 1) resident = 4; });
+    static rb::OncePerDevice once;
+    const cudaError_t counted = once.run(ctx, [](int& blocks) { return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, token_scores_kernel<T>, THREADS, 0); });
+    const int resident = counted == cudaSuccess && once.value[ctx->device] > 0 ? once.value[ctx->device] : 1;
     const uint64_t slots = (uint64_t)ctx->sm_count * resident, bytes = (uint64_t)a.vocab * sizeof(T);
     uint32_t parts = 1;
     if (bytes >= (a.k ? 160u : 96u) * 1024)

@@ -221,3 +221,35 @@ def test_linear_respects_the_sm_limit(client):
         linear_case(client, 4, 1200, 256, BF16, bias=False)
     finally:
         _check(client._lib.rb_set_sm_limit(client._ctx, C.c_int32(0)))
+
+
+def test_more_than_2_to_the_32_values(client):
+    """Offsets beyond 32 bits in every operator: 4.6e9 values, of which the last row is checked."""
+    rows, width = 70000, 65536
+    rng = np.random.default_rng(1)
+    x = client.tensor((rows, width), F16)
+    client.memset(x, 0)
+    last = rng.standard_normal(width).astype(np.float16)
+    client.write(x.handle, last, (rows - 1) * width * 2)
+    client.sync()
+    q, s = RT.quantize_rows(client, x)
+    lq = np.empty(width, np.int8)
+    client.read_into(q.handle, lq, (rows - 1) * width)
+    ls = client.read(s)[-1:]
+    R.check_rows(lq[None], ls, last.astype(np.float64)[None], 2 * 2.0 ** -24, VALUE)
+    w = client.upload(np.ones(width, np.float32))
+    q2, s2 = RT.rms_norm_quant(client, x, w, 1e-5, out=(q,))
+    client.read_into(q.handle, lq, (rows - 1) * width)
+    R.check_rows(lq[None], client.read(s2)[-1:], R.norm(last[None], np.ones(width), 1e-5), NORM_SCALE, VALUE)
+    RT.dequantize_rows(client, q, s2, out=x)
+    back = np.empty(width, np.float16)
+    client.read_into(x.handle, back, (rows - 1) * width * 2)
+    assert np.array_equal(back, (lq.astype(np.float32) * client.read(s2)[-1]).astype(np.float16))
+    del q, q2, s, s2
+    # y of 70000 x 65536 from K = 32: the last rows and columns
+    a, b = rng.integers(-127, 128, (rows, 32)).astype(np.int8), rng.integers(-127, 128, (width, 32)).astype(np.int8)
+    one = lambda n: client.upload(np.ones(n, np.float32))
+    RT.linear_i8(client, client.upload(a), one(rows), client.upload(b), one(width), out=x)
+    client.read_into(x.handle, back, (rows - 1) * width * 2)
+    with np.errstate(over="ignore"):
+        assert np.array_equal(back, (b.astype(np.float32) @ a[-1].astype(np.float32)).astype(np.float16))

@@ -215,3 +215,45 @@ def test_synchronous_context_reports_a_bad_id():
             "except InvalidTensor as e:\n    print('refused:', e)\n")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "refused: token log probabilities: an id is outside" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("scale", [1e-30, 1e-18, 1e-3, 0.02, 50.0, 1e9, 1e18, 1e30])
+def test_scales_far_from_one(client, dtype, scale):
+    """Nearly uniform and nearly certain distributions; all of it in range of FP32 (1e30 times 10 is)."""
+    rng, x, xv, ids = case(4, 3001, dtype)
+    x[1, 2000:] = np.array(-np.inf, np.float32).astype(np.float16).view(x.dtype) if dtype == F16 else (0xff80 if dtype == BF16 else -np.inf)
+    xv = xv.copy()
+    xv[1, 2000:] = -np.inf
+    ids[1] = 5
+    call(client, x, xv, ids, dtype, float(np.float32(scale)), 6)
+
+
+def test_more_than_2_to_the_32_logits(client):
+    """Offsets beyond 32 bits: rows at the end of a batch of 5.2e9 logits, read and written in place."""
+    import ctypes as C
+    from rust_ascend_b200.runtime import _check
+    rows, vocab = 40960, 128000
+    t = client.tensor((rows, vocab), BF16)
+    client.memset(t, 0)
+    ids = np.full(rows, 7, np.int32)
+    rng = np.random.default_rng(0)
+    bits, last = R.hold(rng.standard_normal(vocab) * 2, BF16)
+    client.write(t.handle, bits, (rows - 1) * vocab * 2)
+    client.sync()
+    i = client.upload(ids)
+    out = RT.token_log_probs(client, t, i, top_k=3)
+    want = R.scores(last[None], ids[-1:], 1.0, -100, 3)
+    got = [client.read(o) for o in out]
+    compare([g[-1:] for g in got], want, vocab, 3)
+    even = np.log(vocab)
+    assert np.abs(got[0][:-1] + even).max() < 1e-4 and np.abs(got[2][:-1] - even).max() < 1e-4 and (got[4][:-1] == [0, 1, 2]).all()
+    g = client.upload(np.ones(rows, np.float32))
+    RT.token_log_probs_backward(client, t, i, out[1], out[2], g, out=t)
+    row = np.empty(vocab, np.uint16)
+    client.read_into(t.handle, row, (rows - 1) * vocab * 2)
+    d = R.scores_gradient(last[None], ids[-1:], 1.0, -100, np.ones(1), np.zeros(1))[0]
+    assert np.abs(R.bf16_bits_to_f32(row) - d).max() <= 2.0 ** -8
+    client.read_into(t.handle, row, (rows - 2) * vocab * 2)
+    d = R.bf16_bits_to_f32(row)
+    assert abs(d[7] - (1 - 1 / vocab)) <= 2.0 ** -8 and np.abs(np.delete(d, 7) * vocab + 1).max() <= 2.0 ** -7
