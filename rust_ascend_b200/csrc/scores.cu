@@ -214,6 +214,7 @@ struct Shared {
     Stats mine;                          // this block's part, read by the cluster's first block
     float chunk[CHUNKS][THREADS];        // largest element of each thread's chunks
     uint16_t again[AGAIN];               // chunks to read again: thread + 256 * chunk
+    uint32_t all[WARPS], any[WARPS];     // of the slices' keys
     uint32_t found, again_count;
     uint32_t tie_warp[WARPS];
 };
@@ -254,12 +255,15 @@ __device__ __forceinline__ void merge_lists(Shared& sh, uint32_t lists, uint32_t
     }
 }
 
-// The largest bound of BITS leading bits that k of the block's keys (one per thread) reach; bit by bit from the top.
+// The largest bound of BITS leading bits that k of the block's keys (one per thread) reach, bit by bit from the first in which the
+// keys differ; `all` and `any` are their conjunction and disjunction.
 template <int BITS>
-__device__ __forceinline__ uint32_t kth_of_block(uint32_t key, uint32_t k) {
-    uint32_t bound = 0;
+__device__ __forceinline__ uint32_t kth_of_block(uint32_t key, uint32_t k, uint32_t all, uint32_t any) {
+    const int top = 31 - __clz((int)(all ^ any));             // -1: all alike
+    uint32_t bound = top < 0 ? any : any & ~(0xffffffffu >> (31 - top));
+    if (top < 0) bound &= ~(0xffffffffu >> (BITS - 1) >> 1);
 #pragma unroll 1
-    for (int bit = 31; bit >= 32 - BITS; --bit) {
+    for (int bit = top; bit >= 32 - BITS; --bit) {
         const uint32_t trial = bound | (1u << bit);
         if ((uint32_t)__syncthreads_count(key >= trial) >= k) bound = trial;
     }
@@ -403,6 +407,10 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
 
         Stats st = join_lanes({run.m, run.s0 + run.s1, run.t0 + run.t1}, 32);
         if (lane == 0) sh.warp[tid >> 5] = st;
+        if (a.k) {
+            const uint32_t all = __reduce_and_sync(0xffffffffu, slice_key), any = __reduce_or_sync(0xffffffffu, slice_key);
+            if (lane == 0) { sh.all[tid >> 5] = all; sh.any[tid >> 5] = any; }
+        }
         if (tid == 0) { sh.found = 0; sh.again_count = 0; }
         __syncthreads();
         if (tid < 32) st = join_lanes(sh.warp[lane % WARPS], WARPS);
@@ -410,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
         uint32_t want = 0;
         if (a.k) {
             want = a.k < last - first ? a.k : last - first;
-            const uint32_t bound = kth_of_block<Traits<T>::BOUND_BITS>(slice_key, a.k);
+            const uint32_t bound = kth_of_block<Traits<T>::BOUND_BITS>(slice_key, a.k, __reduce_and_sync(0xffffffffu, sh.all[lane % WARPS]), __reduce_or_sync(0xffffffffu, sh.any[lane % WARPS]));
             if (slice_key >= bound) {
                 const uint32_t mine = (round + (1u << chunk_shift) - 1) >> chunk_shift;
                 for (uint32_t c = 0; c < mine; ++c)
