@@ -103,6 +103,31 @@ struct OncePerDevice {
     }
 };
 
+// Launch that may overlap the end of the work in front of it (programmatic dependent launch): the blocks start when those of the
+// kernel in front have started and said so, or ended, and wait in `predecessor_done` before they touch memory.  Every thread of
+// such a kernel passes that wait, so a kernel never ends before the ones in front of it have.  `cluster` blocks form a cluster (0: what the
+// kernel says).  overlap false: an ordinary launch, for kernels whose blocks share work by their number and count on the placement
+// that an empty GPU gives them.
+// A failure is what after_launch reports.
+template <typename... P, typename... A>
+void launch_behind(rb_ctx* ctx, void (*kernel)(P...), uint64_t grid, unsigned block, size_t smem, unsigned cluster, bool overlap, A&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(block); cfg.dynamicSmemBytes = smem; cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2] = {};
+    unsigned n = 0;
+    if (overlap) { attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[n++].val.programmaticStreamSerializationAllowed = 1; }
+    if (cluster) { attr[n].id = cudaLaunchAttributeClusterDimension; attr[n].val.clusterDim.x = cluster; attr[n].val.clusterDim.y = 1; attr[n++].val.clusterDim.z = 1; }
+    cfg.attrs = attr; cfg.numAttrs = n;
+    cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+#if defined(__CUDACC__)
+// Lets the kernel behind start its blocks, and waits until the work in front has ended and its writes are visible.
+__device__ __forceinline__ void predecessor_done() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+#endif
+
 // Called after every kernel launch: records launch failures on the sticky list, counts the launch
 // and synchronises when the context runs in the reference's synchronous mode.
 int32_t after_launch(rb_ctx* ctx, const char* operation);

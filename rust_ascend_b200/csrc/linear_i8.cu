@@ -110,6 +110,7 @@ template <typename Out, int M, int R>
 __global__ void __launch_bounds__(128) linear_i8_row_kernel(const int8_t* __restrict__ x, const int8_t* __restrict__ w, const LinearParams p, const uint32_t k) {
     constexpr int UNROLL = 4 / R;
     const uint32_t lane = threadIdx.x & 31, row0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * R;
+    rb::predecessor_done();
     if (row0 >= p.n) return;                            // a whole warp
     const uint32_t vectors = k / 16;
     const uint4* at[R];
@@ -212,8 +213,9 @@ linear_i8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         mbar_init(done_bar, 1);
         *abort_word = 0;
         fence_barrier_init();
-        for (uint32_t i = 0; i < ahead; ++i) fetch(kb0 + i, i);
     }
+    rb::predecessor_done();
+    if (threadIdx.x == 0) for (uint32_t i = 0; i < ahead; ++i) fetch(kb0 + i, i);
     if (warp == 1) { tmem_alloc(tmem_slot, C::TMEM_COLS); tmem_relinquish(); }
     for (uint32_t j = threadIdx.x; j < (uint32_t)TOKENS; j += THREADS) sx[j] = j < tokens ? p.sx[token0 + j] : 0.f;
     tc_fence_before();
@@ -346,6 +348,7 @@ linear_i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();
+    rb::predecessor_done();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
@@ -446,12 +449,7 @@ int32_t launch_few(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, u
     CUtensorMap mw, mx;
     if (!byte_map(&mw, w, p.n, k, ROWS) || !byte_map(&mx, x, p.m, k, TOKENS)) return rb::fail(RB_STATUS, "cuTensorMapEncodeTiled failed for the 8-bit linear (m=%u n=%u k=%u)", p.m, p.n, k);
     p.tiles_n = (p.n + ROWS - 1) / ROWS; p.tiles_t = (p.m + TOKENS - 1) / TOKENS;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(p.tiles_n * p.tiles_t * parts); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = Few<TOKENS>::SMEM_BYTES; cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension; attr.val.clusterDim.x = parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr; cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kernel, mw, mx, p);     // a failure is what after_launch reports
+    rb::launch_behind(ctx, kernel, (uint64_t)p.tiles_n * p.tiles_t * parts, THREADS, Few<TOKENS>::SMEM_BYTES, parts, true, mw, mx, p);
     return rb::after_launch(ctx, "8-bit linear (few tokens)");
 }
 
@@ -486,7 +484,7 @@ int32_t launch_pair(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, 
     CUtensorMap mw, mx, mxh;
     if (!byte_map(&mw, w, p.n, k, ROWS) || !byte_map(&mx, x, p.m, k, tokens / 2) || !byte_map(&mxh, x, p.m, k, tokens / 4))
         return rb::fail(RB_STATUS, "cuTensorMapEncodeTiled failed for the 8-bit linear (m=%u n=%u k=%u)", p.m, p.n, k);
-    linear_i8_pair_kernel<Out><<<2 * pairs, THREADS, PAIR_SMEM_BYTES, ctx->stream>>>(mw, mx, mxh, p);
+    rb::launch_behind(ctx, linear_i8_pair_kernel<Out>, 2 * pairs, THREADS, PAIR_SMEM_BYTES, 0, true, mw, mx, mxh, p);
     return rb::after_launch(ctx, "8-bit linear (CTA pairs)");
 }
 
@@ -496,7 +494,7 @@ int32_t launch_rows(rb_ctx* ctx, const LinearParams& p, const void* w, const voi
     // More rows a warp (R) mean fewer loads of x and fewer warps.  us for n x k and m tokens at R = 1 / 2 / 4: 1024 x 4096, 1: 3.0 / 3.7 / 5.3;
     // 6144 x 4096, 1: 6.8 / 5.9 / 7.2; 6144 x 4096, 4: - / 9.1 / 6.9; 4096 x 4096, 4: 6.6 / 6.2 / 6.1.
     const uint32_t sms = (uint32_t)ctx->sm_count;
-#define RB_ROWS(M, R) linear_i8_row_kernel<Out, M, R><<<(p.n + 4 * R - 1) / (4 * R), 128, 0, ctx->stream>>>(xp, wp, p, k)
+#define RB_ROWS(M, R) rb::launch_behind(ctx, linear_i8_row_kernel<Out, M, R>, (p.n + 4 * R - 1) / (4 * R), 128, 0, 0, true, xp, wp, p, k)
     if (p.m == 1) { if (p.n <= 32 * sms) RB_ROWS(1, 1); else RB_ROWS(1, 2); }
     else if (p.m == 2) { if (p.n <= 16 * sms) RB_ROWS(2, 1); else RB_ROWS(2, 2); }
     else { if (p.n <= 32 * sms) RB_ROWS(4, 2); else RB_ROWS(4, 4); }

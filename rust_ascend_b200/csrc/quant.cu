@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
     const uint32_t vectors = a.width / VEC;            // VEC divides the width
     void* mine = s_rows + (size_t)group * a.row_bytes;
     const Weight* weight = static_cast<const Weight*>(a.w);
+    rb::predecessor_done();
     for (uint64_t row = (uint64_t)blockIdx.x * groups + group; row < a.rows; row += (uint64_t)gridDim.x * groups) {
         const In* x = reinterpret_cast<const In*>(static_cast<const T*>(a.x) + row * a.ldx);
         const In* o = reinterpret_cast<const In*>(static_cast<const T*>(a.other) + row * a.ldo);
@@ -361,6 +362,7 @@ __global__ void __launch_bounds__(512, 2) quant_shifted_kernel(const QuantArgs a
     __shared__ float s_most[16];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, threads = blockDim.x, tid = threadIdx.x;
     T* held = reinterpret_cast<T*>(s_rows);
+    rb::predecessor_done();
     for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* x = static_cast<const T*>(a.x) + row * a.ldx;
         const uint32_t to_boundary = (uint32_t)((16u - (reinterpret_cast<uintptr_t>(x) & 15u)) & 15u) / (uint32_t)sizeof(T);
@@ -431,7 +433,7 @@ int32_t launch(rb_ctx* ctx, QuantArgs a, const char* what) {
     a.row_bytes = (a.held * vector_bytes + 15) & ~15u;
     if (a.row_bytes * groups > ROW_SMEM) { a.held -= 16; a.row_bytes = (a.held * vector_bytes + 15) & ~15u; }
     const uint64_t blocks = (a.rows + groups - 1) / groups, cap = 1u << 30;
-    quant_rows_kernel<T, TW, MODE, VEC, UNROLL><<<(unsigned)(blocks < cap ? blocks : cap), groups * warps * 32, a.row_bytes * groups, ctx->stream>>>(a);
+    rb::launch_behind(ctx, quant_rows_kernel<T, TW, MODE, VEC, UNROLL>, blocks < cap ? blocks : cap, groups * warps * 32, a.row_bytes * groups, 0, true, a);
     return rb::after_launch(ctx, what);
 }
 
@@ -444,7 +446,7 @@ int32_t launch_shifted(rb_ctx* ctx, const QuantArgs& a, const char* what) {
     uint32_t warps = (vectors + wanted * 32 - 1) / (wanted * 32);
     if (warps > 16) warps = 16;
     const uint64_t cap = 1u << 30;
-    quant_shifted_kernel<T><<<(unsigned)(a.rows < cap ? a.rows : cap), warps * 32, (a.width * sizeof(T) + 32 + 15) & ~15u, ctx->stream>>>(a);
+    rb::launch_behind(ctx, quant_shifted_kernel<T>, a.rows < cap ? a.rows : cap, warps * 32, (a.width * sizeof(T) + 32 + 15) & ~15u, 0, true, a);
     return rb::after_launch(ctx, what);
 }
 
@@ -495,6 +497,7 @@ __global__ void __launch_bounds__(256, 8) dequant_kernel(const int8_t* q, const 
     typedef Pack<int8_t, PER> Bytes;
     const Index vectors = (Index)(total / PER), base = (Index)blockIdx.x * 256 * UNROLL + threadIdx.x;
     Bytes b[UNROLL];
+    rb::predecessor_done();
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) if (base + u * 256 < vectors) b[u] = streamed(reinterpret_cast<const Bytes*>(q) + base + u * 256);
 #pragma unroll
@@ -533,8 +536,8 @@ template <typename T>
 void launch_dequant(rb_ctx* ctx, const int8_t* q, const float* scales, void* y, uint64_t total, uint32_t width) {
     const uint64_t blocks = (total + 8191) / 8192;
     const unsigned grid = (unsigned)(blocks ? blocks : 1);
-    if (total <= 0xf0000000ull) dequant_kernel<T, uint32_t><<<grid, 256, 0, ctx->stream>>>(q, scales, (T*)y, total, width, divisor(width));
-    else dequant_kernel<T, uint64_t><<<grid, 256, 0, ctx->stream>>>(q, scales, (T*)y, total, width, divisor(width));
+    if (total <= 0xf0000000ull) rb::launch_behind(ctx, dequant_kernel<T, uint32_t>, grid, 256, 0, 0, true, q, scales, (T*)y, total, width, divisor(width));
+    else rb::launch_behind(ctx, dequant_kernel<T, uint64_t>, grid, 256, 0, 0, true, q, scales, (T*)y, total, width, divisor(width));
 }
 
 bool is_float(uint32_t dtype) { return dtype == RB_F32 || dtype == RB_BF16 || dtype == RB_F16; }

@@ -212,3 +212,44 @@ def test_nn_functions(client):
         nn.TokenScoreConfig(temperature=0.0).forward(logits, ids)
     with pytest.raises(InvalidTensor, match="SwiGLU"):
         nn.swiglu_quantized(q, wd, wg)
+
+
+def test_copies_and_other_kernels_between(client):
+    """The operators start their blocks early behind each other; behind a copy, a fill or a kernel that does not take part they still see its
+    result, eagerly and in a recording."""
+    rng = np.random.default_rng(3)
+    rows, width = 64, 2048
+    src, x, y = (client.tensor((rows, width), F32) for _ in range(3))
+    q, s, back = client.tensor((rows, width), I8), client.tensor((rows,), F32), client.tensor((rows, width), F32)
+
+    def sequence():
+        _check(client._lib.rb_copy(client._ctx, C.byref(src._c()), C.byref(x._c())))
+        RT.quantize_rows(client, x, out=(q, s))
+        RT.dequantize_rows(client, q, s, out=back)
+        RT.add(client, back, x, out=y)                    # an ordinary launch
+        RT.quantize_rows(client, y, out=(q, s))
+        client.memset(back, 0)
+        RT.dequantize_rows(client, q, s, out=back)
+
+    def expected(v):
+        def held(a):
+            scale = np.maximum(np.abs(a).max(-1, keepdims=True) / np.float32(127), np.float32(R.SMALLEST))
+            return np.rint(a.astype(np.float64) / scale) * scale
+        return held((held(v).astype(np.float32) + v))
+    sequence()
+    client.sync()
+    _check(client._lib.rb_graph_begin(client._ctx))
+    sequence()
+    g = C.c_uint64()
+    _check(client._lib.rb_graph_end(client._ctx, C.byref(g)))
+    for i in range(6):
+        v = rng.standard_normal((rows, width)).astype(np.float32) * (i + 1)
+        client.write(src.handle, v)
+        if i % 2:
+            _check(client._lib.rb_graph_launch(client._ctx, g))
+        else:
+            sequence()
+        # a value on the border between two steps may fall on either side: one step of the row's scale
+        assert np.abs(client.read(back) - expected(v)).max() <= 1.01 * np.abs(2 * v).max() / 127
+        assert np.mean(np.abs(client.read(back) - expected(v)) > 1e-4) < 1e-3
+    _check(client._lib.rb_graph_destroy(client._ctx, g))
