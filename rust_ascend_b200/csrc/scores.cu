@@ -288,7 +288,7 @@ __device__ uint32_t count_in_block(Shared& sh, const T* row, uint32_t first, uin
 }
 
 // Rows on which the bound lets too many elements through: many equal ones (a masked vocabulary, a constant row) or a hostile order.
-// Takes the elements above the bound, after tightening it to the exact k-th value where they would not fit, then fills up with the
+// `bound` is the k-th largest slice maximum itself, so that equal elements are equal to it.  Takes the elements above it, after tightening it to the exact k-th value where they would not fit, then fills up with the
 // equal ones of lowest index.
 template <typename T>
 __device__ __noinline__ void exact_candidates(Shared& sh, const T* row, uint32_t first, uint32_t last, uint32_t bound, uint32_t want) {
@@ -424,7 +424,8 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
         uint32_t want = 0;
         if (a.k) {
             want = a.k < last - first ? a.k : last - first;
-            const uint32_t bound = kth_of_block<Traits<T>::BOUND_BITS>(slice_key, a.k, __reduce_and_sync(0xffffffffu, sh.all[lane % WARPS]), __reduce_or_sync(0xffffffffu, sh.any[lane % WARPS]));
+            const uint32_t all = __reduce_and_sync(0xffffffffu, sh.all[lane % WARPS]), any = __reduce_or_sync(0xffffffffu, sh.any[lane % WARPS]);
+            const uint32_t bound = kth_of_block<Traits<T>::BOUND_BITS>(slice_key, a.k, all, any);
             if (slice_key >= bound) {
                 const uint32_t mine = (round + (1u << chunk_shift) - 1) >> chunk_shift;
                 for (uint32_t c = 0; c < mine; ++c)
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
                 }
             }
             __syncthreads();
-            if (again > AGAIN || sh.found > CANDIDATES) exact_candidates<T>(sh, row, first, last, bound, want);
+            if (again > AGAIN || sh.found > CANDIDATES) exact_candidates<T>(sh, row, first, last, kth_of_block<32>(slice_key, a.k, all, any), want);
             rank_candidates(sh, sh.found, want);
         }
         if (parts > 1) {

@@ -257,3 +257,20 @@ def test_more_than_2_to_the_32_logits(client):
     client.read_into(t.handle, row, (rows - 2) * vocab * 2)
     d = R.bf16_bits_to_f32(row)
     assert abs(d[7] - (1 - 1 / vocab)) <= 2.0 ** -8 and np.abs(np.delete(d, 7) * vocab + 1).max() <= 2.0 ** -7
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("vocab", [3000, 130000])
+def test_more_ties_than_candidates(client, dtype, vocab):
+    """Thousands of equal logits, positive, negative and masked, around the place where the list ends: the lowest indices win."""
+    rng = np.random.default_rng(vocab)
+    x = np.full((6, vocab), -1.5, np.float32)
+    x[1] = 2.25
+    x[2] = -np.inf
+    x[2, rng.integers(0, vocab, 30)] = rng.standard_normal(30)
+    x[3] = rng.integers(-3, 4, vocab)
+    x[4] = -rng.integers(5, 9, vocab)
+    x[5] = np.where(np.arange(vocab) % 2048 < 1500, -3.0, -4.0)
+    x, xv = R.hold(x, dtype)
+    for top in (1, 20, 64):
+        call(client, x, xv, rng.integers(0, vocab, 6), dtype, 1.0, top)
