@@ -124,6 +124,7 @@ class TensorBuffer:
     strides: tuple = field(default=None)
     offset: int = 0
     _owner: object = field(default=None, repr=False, compare=False)
+    _descriptor = None               # the C descriptor, once made (see _ref)
 
     def __post_init__(self):
         self.shape = tuple(int(d) for d in self.shape)
@@ -167,7 +168,7 @@ class TensorBuffer:
 def _ref(t: TensorBuffer | None):
     if t is None:
         return None
-    d = t.__dict__.get("_descriptor")
+    d = t._descriptor
     if d is None:
         d = t.__dict__["_descriptor"] = C.byref(t._c())
     return d
@@ -362,10 +363,9 @@ class B200Runtime:
     @staticmethod
     def _outputs(out, count: int) -> list:
         """The caller's result tensors, padded with None; more than the operator has is an error."""
-        out = list(out) if out is not None else []
         if len(out) > count:
             raise InvalidTensor(f"at most {count} output tensors are taken")
-        return out + [None] * (count - len(out))
+        return [*out, *(None,) * (count - len(out))]
 
     # -- row programs ----------------------------------------------------------------------------
     @staticmethod
@@ -391,29 +391,35 @@ class B200Runtime:
         """RMSNorm of `input`, or of `input + delta` rounded to the input's type, with its result as I8 rows: rb_rms_norm_quant.
         Returns [q, scales], and the sum as a third entry where `delta` is given.  `out` = (q, scales[, sum]) writes into the
         caller's tensors instead of new ones (the sum may be `input` itself)."""
-        q, scales, total = B200Runtime._outputs(out, 3)
-        q = q or client.tensor(input.shape, DType.I8)
-        scales = scales or client.tensor(input.shape[:-1] or (1,), DType.F32)
+        if out is None:
+            out = (client.tensor(input.shape, DType.I8), client.tensor(input.shape[:-1] or (1,), DType.F32))
+        q, scales, total = out if len(out) == 3 else B200Runtime._outputs(out, 3)
         if delta is not None and total is None:
             total = client.tensor(input.shape, input.dtype)
-        _check(client._lib.rb_rms_norm_quant(client._ctx, _ref(input), _ref(delta), _ref(weight), C.c_double(epsilon), _ref(total), _ref(q), _ref(scales)))
-        return [q, scales] + ([total] if delta is not None else [])
+        code = client._lib.rb_rms_norm_quant(client._ctx, _ref(input), _ref(delta), _ref(weight), C.c_double(epsilon), _ref(total), _ref(q), _ref(scales))
+        if code:
+            _check(code)
+        return [q, scales, total] if delta is not None else [q, scales]
 
     @staticmethod
     def quantize_rows(client: ComputeClient, input: TensorBuffer, up: TensorBuffer | None = None, out=None):
         """[q, scales]: rows of `input`, or of SiLU(input) * up, as I8 with one FP32 scale a row (rb_quantize_rows).  Both inputs may be
         column ranges of wider tensors.  `out` = (q, scales) writes into the caller's tensors."""
-        q, scales = B200Runtime._outputs(out, 2)
-        q = q or client.tensor(input.shape, DType.I8)
-        scales = scales or client.tensor(input.shape[:-1] or (1,), DType.F32)
-        _check(client._lib.rb_quantize_rows(client._ctx, _ref(input), _ref(up), _ref(q), _ref(scales)))
+        if out is None:
+            out = (client.tensor(input.shape, DType.I8), client.tensor(input.shape[:-1] or (1,), DType.F32))
+        q, scales = out if len(out) == 2 else B200Runtime._outputs(out, 2)
+        code = client._lib.rb_quantize_rows(client._ctx, _ref(input), _ref(up), _ref(q), _ref(scales))
+        if code:
+            _check(code)
         return [q, scales]
 
     @staticmethod
     def dequantize_rows(client: ComputeClient, q: TensorBuffer, scales: TensorBuffer, dtype: DType = DType.BF16, out: TensorBuffer | None = None) -> TensorBuffer:
         """q * scale of its row, in `dtype` or in the type of `out` (rb_dequantize_rows)."""
         out = out or client.tensor(q.shape, dtype)
-        _check(client._lib.rb_dequantize_rows(client._ctx, _ref(q), _ref(scales), _ref(out)))
+        code = client._lib.rb_dequantize_rows(client._ctx, _ref(q), _ref(scales), _ref(out))
+        if code:
+            _check(code)
         return out
 
     @staticmethod
@@ -424,7 +430,9 @@ class B200Runtime:
         if len(weight.shape) != 2 or not input.shape:
             raise InvalidTensor("8-bit linear takes X[..,K] and W[N,K]")
         out = out or client.tensor(input.shape[:-1] + (weight.shape[0],), dtype)
-        _check(client._lib.rb_linear_i8(client._ctx, _ref(input), _ref(input_scales), _ref(weight), _ref(weight_scales), _ref(bias), _ref(out)))
+        code = client._lib.rb_linear_i8(client._ctx, _ref(input), _ref(input_scales), _ref(weight), _ref(weight_scales), _ref(bias), _ref(out))
+        if code:
+            _check(code)
         return out
 
     # -- scores of single tokens (no counterpart in the reference) -----------------------------------------------------
@@ -433,15 +441,17 @@ class B200Runtime:
         """[log_probs, lse, entropy, top_values, top_ids] of rows of logits [.., V] scaled by `scale` (one over the temperature):
         rb_token_log_probs.  The last two are None when top_k is 0.  `out` takes the five tensors in that order; entropy may be
         None there to leave it out."""
-        rows = logits.shape[:-1] or (1,)
-        if out is None:
-            out = [client.tensor(rows, DType.F32) for _ in range(3)]
-            out += [client.tensor(rows + (top_k,), DType.F32), client.tensor(rows + (top_k,), DType.I32)] if top_k else [None, None]
-        log_probs, lse, entropy, top_values, top_ids = B200Runtime._outputs(out, 5)
         if not 0 <= top_k <= 64:
             raise InvalidTensor("top_k must be within 0..64 and the vocabulary")
-        _check(client._lib.rb_token_log_probs(client._ctx, _ref(logits), _ref(ids), C.c_float(scale), C.c_int64(ignore_index), _ref(log_probs), _ref(lse),
-                                              _ref(entropy), C.c_uint32(top_k), _ref(top_values), _ref(top_ids)))
+        if out is None:
+            rows = logits.shape[:-1] or (1,)
+            out = [client.tensor(rows, DType.F32) for _ in range(3)]
+            out += [client.tensor(rows + (top_k,), DType.F32), client.tensor(rows + (top_k,), DType.I32)] if top_k else [None, None]
+        log_probs, lse, entropy, top_values, top_ids = out if len(out) == 5 else B200Runtime._outputs(out, 5)
+        code = client._lib.rb_token_log_probs(client._ctx, _ref(logits), _ref(ids), C.c_float(scale), C.c_int64(ignore_index), _ref(log_probs), _ref(lse),
+                                              _ref(entropy), C.c_uint32(top_k), _ref(top_values), _ref(top_ids))
+        if code:
+            _check(code)
         return [log_probs, lse, entropy, top_values, top_ids]
 
     @staticmethod
@@ -451,8 +461,10 @@ class B200Runtime:
         """Gradient of token_log_probs with respect to the logits from the saved lse and entropy (rb_token_log_probs_backward); `out`
         may be `logits` itself."""
         out = out or client.tensor(logits.shape, logits.dtype)
-        _check(client._lib.rb_token_log_probs_backward(client._ctx, _ref(logits), _ref(ids), C.c_float(scale), C.c_int64(ignore_index), _ref(lse),
-                                                       _ref(entropy), _ref(grad_log_probs), _ref(grad_entropy), _ref(out)))
+        code = client._lib.rb_token_log_probs_backward(client._ctx, _ref(logits), _ref(ids), C.c_float(scale), C.c_int64(ignore_index), _ref(lse),
+                                                       _ref(entropy), _ref(grad_log_probs), _ref(grad_entropy), _ref(out))
+        if code:
+            _check(code)
         return out
 
     @staticmethod
