@@ -390,10 +390,12 @@ class B200Runtime:
     def rms_norm_quant(client: ComputeClient, input: TensorBuffer, weight: TensorBuffer, epsilon: float, delta: TensorBuffer | None = None, out=None):
         """RMSNorm of `input`, or of `input + delta` rounded to the input's type, with its result as I8 rows: rb_rms_norm_quant.
         Returns [q, scales], and the sum as a third entry where `delta` is given.  `out` = (q, scales[, sum]) writes into the
-        caller's tensors instead of new ones (the sum may be `input` itself)."""
-        if out is None:
-            out = (client.tensor(input.shape, DType.I8), client.tensor(input.shape[:-1] or (1,), DType.F32))
-        q, scales, total = out if len(out) == 3 else B200Runtime._outputs(out, 3)
+        caller's tensors instead of new ones (the sum may be `input` itself); what is missing or None there is made."""
+        q, scales, total = out if out is not None and len(out) == 3 else B200Runtime._outputs(out or (), 3)
+        if q is None:
+            q = client.tensor(input.shape, DType.I8)
+        if scales is None:
+            scales = client.tensor(input.shape[:-1] or (1,), DType.F32)
         if delta is not None and total is None:
             total = client.tensor(input.shape, input.dtype)
         code = client._lib.rb_rms_norm_quant(client._ctx, _ref(input), _ref(delta), _ref(weight), C.c_double(epsilon), _ref(total), _ref(q), _ref(scales))
@@ -405,9 +407,11 @@ class B200Runtime:
     def quantize_rows(client: ComputeClient, input: TensorBuffer, up: TensorBuffer | None = None, out=None):
         """[q, scales]: rows of `input`, or of SiLU(input) * up, as I8 with one FP32 scale a row (rb_quantize_rows).  Both inputs may be
         column ranges of wider tensors.  `out` = (q, scales) writes into the caller's tensors."""
-        if out is None:
-            out = (client.tensor(input.shape, DType.I8), client.tensor(input.shape[:-1] or (1,), DType.F32))
-        q, scales = out if len(out) == 2 else B200Runtime._outputs(out, 2)
+        q, scales = out if out is not None and len(out) == 2 else B200Runtime._outputs(out or (), 2)
+        if q is None:
+            q = client.tensor(input.shape, DType.I8)
+        if scales is None:
+            scales = client.tensor(input.shape[:-1] or (1,), DType.F32)
         code = client._lib.rb_quantize_rows(client._ctx, _ref(input), _ref(up), _ref(q), _ref(scales))
         if code:
             _check(code)
