@@ -156,16 +156,17 @@ __device__ __forceinline__ float largest(const Vec<T> (&x)[U]) {
         return max_nan(to_f32(top.x), to_f32(top.y));
     }
 }
-// Two neighbouring elements, lifted to `low` (NaN too: the reference has it), as FP32.
+// Two neighbouring elements, lifted to `low` (NaN too: the reference has it), as FP32.  `low` rounds down into the storage type: rounded up it
+// could pass the row's own largest element (steps of 4096 at a million in BF16).
 template <typename T>
 __device__ __forceinline__ void lifted(const T* p, float low, float& a, float& b) {
     if constexpr (sizeof(T) == 4) { a = fmaxf(p[0], low); b = fmaxf(p[1], low); }
     else if constexpr (std::is_same<T, bf>::value) {
-        const __nv_bfloat162 x = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(p), __float2bfloat162_rn(low));
+        const __nv_bfloat162 x = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(p), __bfloat162bfloat162(__float2bfloat16_rd(low)));
         const uint32_t w = *reinterpret_cast<const uint32_t*>(&x);
         a = __uint_as_float(w << 16); b = __uint_as_float(w & 0xffff0000u);
     } else {
-        const float2 f = __half22float2(__hmax2(*reinterpret_cast<const __half2*>(p), __float2half2_rn(low)));
+        const float2 f = __half22float2(__hmax2(*reinterpret_cast<const __half2*>(p), __half2half2(__float2half_rd(low))));
         a = f.x; b = f.y;
     }
 }

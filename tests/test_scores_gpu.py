@@ -274,3 +274,26 @@ def test_more_ties_than_candidates(client, dtype, vocab):
     x, xv = R.hold(x, dtype)
     for top in (1, 20, 64):
         call(client, x, xv, rng.integers(0, vocab, 6), dtype, 1.0, top)
+
+
+@pytest.mark.parametrize("dtype,scale,top", [(BF16, 1.0, 1003520.0), (BF16, 1.0, -1003520.0), (BF16, 1.0, 266240.0), (BF16, 0.25, -2129920.0), (F16, 64.0, 65504.0),
+                                             (F32, 1.0, 1003520.0), (F32, 64.0, -65504.0)])
+def test_gradient_of_certain_rows_far_from_zero(client, dtype, scale, top):
+    """One logit far above all others, and lse so large that neighbouring values of the type are hundreds apart: p is 1 there and 0 everywhere
+    else, to the bit.  Where it is 1 it inherits the rounding of lse log2(e) (2^-24) and of lse (2^-24, exact here), and the exponential's 2^-22."""
+    vocab = 1001
+    x = np.full((2, vocab), top - abs(top) / 64)
+    x[:, 77] = top
+    x[:, 5] = -top if top > 0 else 1.5 * top
+    x, xv = R.hold(x, dtype)
+    assert xv[0, 77] == top and np.sort(xv[0])[-2] < top
+    lse = np.full(2, top * scale, np.float32)
+    ids, g, h = np.array([77, 300]), np.array([2, 2], np.float32), np.array([0, 1], np.float32)
+    up = client.upload
+    d = R.read(client, RT.token_log_probs_backward(client, up(x, dtype), up(ids), up(lse), up(np.zeros(2, np.float32)), up(g), up(h), scale=scale)).astype(np.float64) / scale
+    others = np.ones(vocab, bool)
+    others[[77, 300]] = False
+    assert not d[:, others].any() and d[0, 300] == 0 and d[1, 300] == 2
+    # d of the largest: within e of 0, p within exp(e ln 2), and h p log p within h e
+    e = 2 * abs(top * scale) * U + 2.0 ** -20
+    assert abs(d[0, 77]) <= 2 * np.expm1(e) and abs(d[1, 77] + 2) <= (2 + e) * np.exp(e) * (1 + R.half_step(dtype)) - 2 + 4 * U
