@@ -332,7 +332,8 @@ RB_API int32_t rb_gemm_no_alloc(rb_ctx* ctx, const rb_tensor* a, const rb_tensor
 /* This entry has no counterpart in the reference.  rb_rms_norm (delta NULL, x_out NULL) or rb_add_rms_norm (both given: the sum
  * is rounded to x's type and stored to x_out, which may be x itself) whose result leaves in 8 bits: y = s * rsqrt(mean(s^2) +
  * epsilon) * w is quantised by rows into q (I8, x's shape) and scales (FP32, one value per row).  x F32, BF16 or F16, any width;
- * weight in x's type or F32.  One pass over x: the normalised row is never stored. */
+ * weight in x's type or F32.  One pass over x: the normalised row is never stored.  The products s * w are formed in FP32 before the
+ * root is divided out: a row in which one leaves FP32's range counts as one that holds an infinity. */
 RB_API int32_t rb_rms_norm_quant(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* delta, const rb_tensor* weight, double epsilon,
                                  const rb_tensor* x_out, const rb_tensor* q, const rb_tensor* scales);
 /* This entry has no counterpart in the reference.  Quantises rows: y = x, or, with `up` given, y = SiLU(x) * up in FP32 (the

@@ -217,6 +217,8 @@ linear_i8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     }
     rb::predecessor_done();
     if (threadIdx.x == 0) for (uint32_t i = 0; i < ahead; ++i) fetch(kb0 + i, i);
+    // Blocks of the kernel behind may be on the SM by now.  Shared memory lets two such CTAs share it (at most 256 of the 512 columns)
+    // and none of the pair kernel's, so nobody that waits for this kernel can hold what it waits for here.
     if (warp == 1) { tmem_alloc(tmem_slot, C::TMEM_COLS); tmem_relinquish(); }
     for (uint32_t j = threadIdx.x; j < (uint32_t)TOKENS; j += THREADS) sx[j] = j < tokens ? p.sx[token0 + j] : 0.f;
     tc_fence_before();

@@ -430,8 +430,7 @@ int32_t launch(rb_ctx* ctx, QuantArgs a, const char* what) {
     const uint32_t groups = warps == 1 ? 8 : 1;
     const uint32_t vector_bytes = VEC * sizeof(H), most_held = ROW_SMEM / groups / vector_bytes;
     a.held = vectors < most_held ? vectors : most_held;
-    a.row_bytes = (a.held * vector_bytes + 15) & ~15u;
-    if (a.row_bytes * groups > ROW_SMEM) { a.held -= 16; a.row_bytes = (a.held * vector_bytes + 15) & ~15u; }
+    a.row_bytes = (a.held * vector_bytes + 15) & ~15u;      // within ROW_SMEM / groups, a multiple of 16 and of every vector_bytes
     const uint64_t blocks = (a.rows + groups - 1) / groups, cap = 1u << 30;
     rb::launch_behind(ctx, quant_rows_kernel<T, TW, MODE, VEC, UNROLL>, blocks < cap ? blocks : cap, groups * warps * 32, a.row_bytes * groups, 0, true, a);
     return rb::after_launch(ctx, what);

@@ -115,13 +115,14 @@ int32_t resolve_rows(rb_ctx* ctx, const rb_tensor* t, const char* what, Rows* ou
         if (it == ctx->storage.end()) return fail(RB_NULL_HANDLE, "%s: unknown storage handle %llu", what, (unsigned long long)t->handle);
         s = it->second;
     }
-    if (t->offset > s.bytes) return fail(RB_INVALID_TENSOR, "%s: strides reach outside the storage", what);
-    uint64_t bytes = 0;
-    if (!empty) {
-        const uint64_t room = (s.bytes - t->offset) / es;
-        if (width > room || (rows > 1 && ld > (room - width) / (rows - 1))) return fail(RB_INVALID_TENSOR, "%s: strides reach outside the storage", what);
-        bytes = ((rows - 1) * ld + width) * es;
+    if (empty) {      // nothing is read: a column range of a tensor without rows may start behind its storage
+        out->ptr = s.ptr; out->rows = rows; out->width = width; out->ld = ld;
+        return RB_OK;
     }
+    if (t->offset > s.bytes) return fail(RB_INVALID_TENSOR, "%s: strides reach outside the storage", what);
+    const uint64_t room = (s.bytes - t->offset) / es;
+    if (width > room || (rows > 1 && ld > (room - width) / (rows - 1))) return fail(RB_INVALID_TENSOR, "%s: strides reach outside the storage", what);
+    const uint64_t bytes = ((rows - 1) * ld + width) * es;
     char* p = (char*)s.ptr + t->offset;
     if (((uintptr_t)p) % es) return fail(RB_INVALID_TENSOR, "%s: device address must be aligned to its element", what);
     out->ptr = p; out->rows = rows; out->width = width; out->ld = ld; out->extent_bytes = bytes;

@@ -375,9 +375,10 @@ def swiglu_quantized(input: QuantizedRows, gate_up: QuantizedRows, down: Quantiz
     """(SiLU(X Wg^T) * (X Wu^T)) Wd^T with all products on 8-bit integers.  gate_up [2 H, K] holds the gate's rows and then the up
     projection's; its product stays in BF16 and is quantised behind SiLU * up where it lies."""
     c = _same_client(input.values, gate_up.values, down.values)
-    rows, hidden = gate_up.dims()[0], down.dims()[1]
-    if len(input.dims()) != 2 or rows != 2 * hidden:
+    shapes = input.dims(), gate_up.dims(), down.dims()
+    if any(len(d) != 2 for d in shapes) or shapes[1][0] != 2 * shapes[2][1]:
         raise InvalidTensor("8-bit SwiGLU requires X[M,K], gate and up stacked as [2 H,K] and down[N,H]")
+    rows, hidden = shapes[1][0], shapes[2][1]
     both = linear_quantized(input, gate_up).buffer
     half = lambda at: TensorBuffer(both.handle, (both.shape[0], hidden), DType.BF16, (rows, 1), both.offset + at * 2, both._owner)
     return linear_quantized(_quantized(c, RT.quantize_rows(c, half(0), up=half(hidden))), down, dtype=dtype)

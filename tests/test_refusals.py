@@ -164,6 +164,26 @@ def test_empty_batches_return_without_a_launch(host):
     assert after["empty_calls"] == before["empty_calls"] + 6 and after["launches"] == before["launches"]
 
 
+def test_column_ranges_of_an_empty_batch(host):
+    """A range of the columns of a tensor without rows starts behind its storage, which nothing reads."""
+    t = host.tensor
+    both = t((0, 128), BF16)
+    half = lambda at: TensorBuffer(both.handle, (0, 64), BF16, (128, 1), both.offset + at * 2)
+    before = host.stats()
+    RT.quantize_rows(host, half(0), up=half(64), out=(t((0, 64), I8), t((0,), F32)))
+    RT.token_log_probs(host, half(64), t((0,), I32), out=[t((0,), F32) for _ in range(3)])
+    assert host.stats()["empty_calls"] == before["empty_calls"] + 2
+    refused("outside the storage", RT.quantize_rows, host, TensorBuffer(both.handle, (1, 64), BF16, None, 128), out=(t((1, 64), I8), t((1,), F32)))
+
+
+def test_swiglu_shapes(host):
+    from rust_ascend_b200 import nn
+    pair = lambda n, k: nn.QuantizedRows(nn.Tensor(host, host.tensor((n, k), I8)), nn.Tensor(host, host.tensor((n,), F32)))
+    flat = nn.QuantizedRows(nn.Tensor(host, host.tensor((64,), I8)), nn.Tensor(host, host.tensor((1,), F32)))
+    for x, gate_up, down in ((flat, pair(96, 64), pair(32, 48)), (pair(4, 64), pair(95, 64), pair(32, 48)), (pair(4, 64), flat, pair(32, 48)), (pair(4, 64), pair(96, 64), flat)):
+        refused("SwiGLU", nn.swiglu_quantized, x, gate_up, down)
+
+
 def test_descriptor_follows_the_fields():
     """The C descriptor of a tensor is made once and dropped when a field changes."""
     import copy
