@@ -122,6 +122,8 @@ void launch_behind(rb_ctx* ctx, void (*kernel)(P...), uint64_t grid, unsigned bl
 }
 #if defined(__CUDACC__)
 // Lets the kernel behind start its blocks, and waits until the work in front has ended and its writes are visible.
+// To ordinary loads, that is: what the work in front may have written is not read through the read-only path (ld.global.nc, __ldg), whose
+// memory has to keep still from the kernel's start on.
 __device__ __forceinline__ void predecessor_done() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -107,7 +107,7 @@ __device__ __forceinline__ void put(const LinearParams& p, uint32_t token, uint3
 // L1) serves R times, and has four to eight vectors of 16 bytes a lane in flight: the next round's loads leave before this round's
 // products.  6144 x 4096, one token: 5.9 us = 4.2 TB/s with the launch; 14336 x 4096: 10.8 us = 5.4 TB/s.
 template <typename Out, int M, int R>
-__global__ void __launch_bounds__(128) linear_i8_row_kernel(const int8_t* __restrict__ x, const int8_t* __restrict__ w, const LinearParams p, const uint32_t k) {
+__global__ void __launch_bounds__(128) linear_i8_row_kernel(const int8_t* x, const int8_t* w, const LinearParams p, const uint32_t k) {
     constexpr int UNROLL = 4 / R;
     const uint32_t lane = threadIdx.x & 31, row0 = (blockIdx.x * 4 + (threadIdx.x >> 5)) * R;
     rb::predecessor_done();
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(128) linear_i8_row_kernel(const int8_t* __rest
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 a[r][u] = make_uint4(0, 0, 0, 0);       // behind the row: adds nothing
-                if (i < vectors) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a[r][u].x), "=r"(a[r][u].y), "=r"(a[r][u].z), "=r"(a[r][u].w) : "l"(at[r] + i));
+                if (i < vectors) asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a[r][u].x), "=r"(a[r][u].y), "=r"(a[r][u].z), "=r"(a[r][u].w) : "l"(at[r] + i));
             }
         }
     };
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(128) linear_i8_row_kernel(const int8_t* __rest
             const uint32_t i = base + u * 32 < vectors ? base + u * 32 : 0;
 #pragma unroll
             for (int t = 0; t < M; ++t) {
-                const uint4 b = __ldg(reinterpret_cast<const uint4*>(x + (size_t)((uint32_t)t < p.m ? t : 0) * k) + i);      // a missing token repeats the first
+                const uint4 b = reinterpret_cast<const uint4*>(x + (size_t)((uint32_t)t < p.m ? t : 0) * k)[i];      // a missing token repeats the first
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     acc[r][t] = __dp4a((int)a[r][u].x, (int)b.x, acc[r][t]);

@@ -26,20 +26,6 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return
 // VEC neighbouring elements: VEC * sizeof(T) is a power of two up to 32 bytes, and addresses are aligned to it or to 16.
 template <typename T, int VEC> struct __align__(VEC * sizeof(T) > 16 ? 16 : VEC * sizeof(T)) Pack { T v[VEC]; };
 
-// A vector that nothing writes while the kernel runs: its load may move in front of stores.
-template <typename P> __device__ __forceinline__ P constant(const P* at) {
-    P p;
-    if constexpr (sizeof(P) % 16 == 0) {
-        uint4 t[sizeof(P) / 16];
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(P) / 16); ++i) t[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
-        memcpy(&p, t, sizeof(P));
-    } else if constexpr (sizeof(P) == 8) { const uint2 t = __ldg(reinterpret_cast<const uint2*>(at)); memcpy(&p, &t, 8); }
-    else if constexpr (sizeof(P) == 4) { const uint32_t t = __ldg(reinterpret_cast<const uint32_t*>(at)); memcpy(&p, &t, 4); }
-    else { const uint16_t t = __ldg(reinterpret_cast<const uint16_t*>(at)); memcpy(&p, &t, 2); }
-    return p;
-}
-
 // Two FP32 operations in one instruction, each rounded as the single one is.
 __device__ __forceinline__ void mul2(float& a, float& b, float x, float y) {
     asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}" : "+f"(a), "+f"(b) : "f"(x), "f"(y));
@@ -270,9 +256,9 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
             for (int u = 0; u < UNROLL; ++u) {
                 const uint32_t i = base + u * threads;
                 const uint32_t at = decltype(whole)::value || i < vectors ? i : vectors - 1;      // behind the row: the last vector again, not used
+                if (NORMS) wt[NORMS ? u : 0] = weight[at];
                 in[u] = x[at];
                 if (TWO) in2[TWO ? u : 0] = o[at];
-                if (NORMS) wt[NORMS ? u : 0] = constant(weight + at);
             }
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
@@ -304,6 +290,7 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
         for (; base + (UNROLL - 1) * threads < vectors; base += UNROLL * threads) chunk(base, std::true_type());
         if (base < vectors) chunk(base, std::false_type());
 
+        constexpr int AHEAD = NORMS && sizeof(Weight) > 16 ? 2 : 4;
         // magnitudes compare as integers, and in that order NaN lies above infinity
         uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
         float sum = sum0 + sum1;
@@ -326,7 +313,7 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
         const Factor f = factor_of<NORMS>(a, row, bits, sum, tid == 0);
         const float c = f.c;
         const bool bad = f.bad, raise = f.raise;
-        auto finish = [&](uint32_t i, auto plain) {
+        auto finish = [&](uint32_t i, const Weight& by, auto plain) {
             float v[VEC];
             [[maybe_unused]] float w[VEC];
             if (i < a.held) widen<H, VEC>(Hold::get(mine, a.held, i), v);
@@ -334,7 +321,7 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
                 widen<T, VEC>(MODE == ADD_NORM ? xo[i] : x[i], v);
                 if constexpr (MODE == GATED) { widen<T, VEC>(o[i], w); silu_mul<VEC>(v, w); }
             }
-            if constexpr (NORMS) { widen<TW, VEC>(constant(weight + i), w); times<VEC>(v, w); }
+            if constexpr (NORMS) { widen<TW, VEC>(by, w); times<VEC>(v, w); }
             if (!decltype(plain)::value) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) v[j] = bad ? 0.f : (raise ? __fmul_rn(v[j], 7.9228163e28f) : v[j]);
@@ -342,11 +329,19 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
             q[i] = to_bytes<VEC>(v, !decltype(plain)::value && bad ? 0.f : c);
         };
         if (!bad && !raise) {
-#pragma unroll 4
-            for (uint32_t i = tid; i < vectors; i += threads) finish(i, std::true_type());
+            // the weights of a few vectors in front of those vectors' stores, which a load may not pass (8192 x 4096: one by one 54 us instead of 37)
+            uint32_t i = tid;
+            for (; i + (AHEAD - 1) * threads < vectors; i += AHEAD * threads) {
+                Weight by[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) if (NORMS) by[u] = weight[i + u * threads];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) finish(i + u * threads, by[u], std::true_type());
+            }
+            for (; i < vectors; i += threads) { Weight by; if (NORMS) by = weight[i]; finish(i, by, std::true_type()); }
         } else {
 #pragma unroll 1
-            for (uint32_t i = tid; i < vectors; i += threads) finish(i, std::false_type());
+            for (uint32_t i = tid; i < vectors; i += threads) { Weight by; if (NORMS) by = weight[i]; finish(i, by, std::false_type()); }
         }
     }
 }
@@ -495,17 +490,29 @@ __global__ void __launch_bounds__(256, 8) dequant_kernel(const int8_t* q, const 
     constexpr int PER = 16 / sizeof(T), UNROLL = 32 / PER;         // 32 elements a thread
     typedef Pack<int8_t, PER> Bytes;
     const Index vectors = (Index)(total / PER), base = (Index)blockIdx.x * 256 * UNROLL + threadIdx.x;
-    Bytes b[UNROLL];
-    rb::predecessor_done();
+    Index rows[UNROLL];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) if (base + u * 256 < vectors) b[u] = streamed(reinterpret_cast<const Bytes*>(q) + base + u * 256);
+    for (int u = 0; u < UNROLL; ++u) rows[u] = divide((base + u * 256) * PER, by_width);
+    Bytes b[UNROLL];
+    float scale[UNROLL];
+    rb::predecessor_done();
+    // every load in front of the stores, which they may not pass
+    if (base + (UNROLL - 1) * 256 < vectors) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) b[u] = streamed(reinterpret_cast<const Bytes*>(q) + base + u * 256);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) scale[u] = scales[rows[u]];
+    } else {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) if (base + u * 256 < vectors) { b[u] = streamed(reinterpret_cast<const Bytes*>(q) + base + u * 256); scale[u] = scales[rows[u]]; }
+    }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         const Index v = base + u * 256;
         if (v >= vectors) break;
-        const Index row = divide(v * PER, by_width);
+        const Index row = rows[u];
         uint32_t col = (uint32_t)(v * PER - row * (Index)width);
-        const float s = __ldg(scales + row);
+        const float s = scale[u];
         float f[PER], by[PER];
         uint32_t word[PER / 4];
         memcpy(word, &b[u], PER);
@@ -518,7 +525,7 @@ __global__ void __launch_bounds__(256, 8) dequant_kernel(const int8_t* q, const 
         if (col + PER > width) {
             Index r = row;
 #pragma unroll
-            for (int j = 1; j < PER; ++j) { if (++col == width) { col = 0; ++r; } by[j] = __ldg(scales + r); }
+            for (int j = 1; j < PER; ++j) { if (++col == width) { col = 0; ++r; } by[j] = scales[r]; }
         }
 #pragma unroll
         for (int j = 0; j < PER; j += 2) add2(f[j], f[j + 1], -8388736.0f, -8388736.0f);

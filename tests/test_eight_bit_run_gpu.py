@@ -214,6 +214,48 @@ def test_nn_functions(client):
         nn.swiglu_quantized(q, wd, wg)
 
 
+def test_every_operand_from_the_kernel_in_front(client):
+    """Activations, scales, weights of the norm and of the linear, logits and saved statistics: each rewritten by the call right in front of
+    the one that reads it, after an earlier call has read the same addresses.  The results are those of calls that wait for each other."""
+    rng = np.random.default_rng(21)
+    rows, k, n = 3, 1024, 640                              # 3 tokens: the linear that reads its operands with ordinary loads
+    t = client.tensor
+    source = [client.upload((rng.standard_normal((n, k)) * (1 + i)).astype(np.float32)) for i in range(4)]
+    x = t((rows, k), F32)
+    w8, ws, xq, xs, nq, ns = t((n, k), I8), t((n,), F32), t((rows, k), I8), t((rows,), F32), t((1, k), I8), t((1,), F32)
+    weight, y = t((k,), F32), t((rows, n), F32)
+    ids = client.upload(rng.integers(0, n, rows))
+    scores, g, d = [t((rows,), F32) for _ in range(3)], client.upload(np.ones(rows, np.float32)), t((rows, n), F32)
+    part = lambda b, first, m: TensorBuffer(b.handle, (m, k), F32, None, first * k * 4, b._owner)
+
+    def round_of(i, wait):
+        out = []
+        done = client.sync if wait else lambda: None
+        s = source[i % 4]
+        RT.quantize_rows(client, part(s, 7, 1), out=(nq, ns)); done()
+        RT.dequantize_rows(client, nq, ns, out=TensorBuffer(weight.handle, (1, k), F32)); done()
+        RT.rms_norm_quant(client, part(s, 8, rows), weight, 1e-5, out=(xq, xs)); done()             # weight from the call in front
+        RT.dequantize_rows(client, xq, xs, out=x); done()
+        RT.quantize_rows(client, s, out=(w8, ws)); done()
+        RT.linear_i8(client, xq, xs, w8, ws, out=y); done()                                         # W and its scales too
+        RT.quantize_rows(client, x, out=(xq, xs)); done()
+        RT.linear_i8(client, xq, xs, w8, ws, out=y); done()                                         # x and its scales
+        RT.token_log_probs(client, y, ids, out=[*scores, None, None]); done()
+        RT.token_log_probs_backward(client, y, ids, scores[1], scores[2], g, g, out=d); done()
+        RT.rms_norm_quant(client, x, weight, 1e-5, delta=part(s, 30, rows), out=(xq, xs, x)); done()
+        for a in (xq, xs, x, y, d, weight):
+            copy = t(a.shape, a.dtype)
+            _check(client._lib.rb_copy(client._ctx, C.byref(a._c()), C.byref(copy._c())))
+            out.append(copy)
+        return out
+    want = [[client.read(a) for a in round_of(i, True)] for i in range(4)]
+    got = [round_of(i, False) for i in range(40)]
+    client.sync()
+    for i, out in enumerate(got):
+        for a, b in zip(out, want[i % 4]):
+            assert np.array_equal(client.read(a), b)
+
+
 def test_copies_and_other_kernels_between(client):
     """The operators start their blocks early behind each other; behind a copy, a fill or a kernel that does not take part they still see its
     result, eagerly and in a recording."""
