@@ -305,7 +305,9 @@ __device__ __noinline__ void exact_candidates(Shared& sh, const T* row, uint32_t
     __syncthreads();
     for (uint32_t i = first + threadIdx.x; i < last; i += THREADS) { const uint32_t key = order_key(to_f32(row[i])); if (key > bound) push(sh, key, i); }
     __syncthreads();
-    uint32_t have = sh.found;                         // at most CANDIDATES by the search above; want - 1 at most where it tightened the bound
+    // At most CANDIDATES by the count above, want - 1 where it tightened the bound.  Held to that for a row that somebody writes meanwhile,
+    // whose scores mean nothing but whose count must not leave the table.
+    uint32_t have = sh.found < (uint32_t)CANDIDATES ? sh.found : CANDIDATES;
     for (uint32_t base = first; base < last && have < want; base += THREADS) {      // all threads see the same `have`
         const uint32_t i = base + threadIdx.x;
         const bool tie = i < last && order_key(to_f32(row[i])) == bound;
@@ -321,7 +323,7 @@ __device__ __noinline__ void exact_candidates(Shared& sh, const T* row, uint32_t
         have += total;
     }
     __syncthreads();
-    if (threadIdx.x == 0 && sh.found < want) sh.found = have < want ? have : want;
+    if (threadIdx.x == 0) sh.found = sh.found < want ? (have < want ? have : want) : (sh.found < (uint32_t)CANDIDATES ? sh.found : CANDIDATES);
     __syncthreads();
 }
 

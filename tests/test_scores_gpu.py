@@ -297,3 +297,31 @@ def test_gradient_of_certain_rows_far_from_zero(client, dtype, scale, top):
     # d of the largest: within e of 0, p within exp(e ln 2), and h p log p within h e
     e = 2 * abs(top * scale) * U + 2.0 ** -20
     assert abs(d[0, 77]) <= 2 * np.expm1(e) and abs(d[1, 77] + 2) <= (2 + e) * np.exp(e) * (1 + R.half_step(dtype)) - 2 + 4 * U
+
+
+def test_rows_written_meanwhile_leave_everything_else_alone(client):
+    """Logits that another stream overwrites during the call, ties by random values and back: the scores of that call mean nothing, but it
+    stays within its tables and tensors, and the next call is right."""
+    import ctypes as C
+    from rust_ascend_b200.runtime import _check
+    rng = np.random.default_rng(8)
+    rows, vocab, top = 150, 40000, 20
+    xv = rng.standard_normal((rows, vocab)).astype(np.float32)
+    ids = rng.integers(0, vocab, rows)
+    ties, values, x, i = client.upload(np.zeros_like(xv)), client.upload(xv), client.upload(np.zeros_like(xv)), client.upload(ids)
+    out = [client.tensor((rows,), F32) for _ in range(3)] + [client.tensor((rows, top), F32), client.tensor((rows, top), I32)]
+    lib, ctx = client._lib, client._ctx
+
+    def copy(a):
+        _check(lib.rb_copy(ctx, C.byref(a._c()), C.byref(x._c())))
+    for n in range(40):
+        _check(lib.rb_aux_begin(ctx))
+        copy(ties if n % 2 else values)
+        _check(lib.rb_aux_end(ctx, C.c_uint32(0)))
+        RT.token_log_probs(client, x, i, top_k=top, out=out)
+        _check(lib.rb_aux_wait(ctx, C.c_uint32(0)))
+    client.sync()
+    copy(values)
+    RT.token_log_probs(client, x, i, top_k=top, out=out)
+    compare([client.read(o) for o in out], R.scores(xv, ids, 1.0, -100, top), vocab, top)
+    assert not client.read(ties).any() and np.array_equal(client.read(values), xv)
