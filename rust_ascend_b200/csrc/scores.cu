@@ -27,21 +27,16 @@ namespace {
 
 using bf = __nv_bfloat16;
 
-constexpr int THREADS = 256;
-constexpr int WARPS = THREADS / 32;
+constexpr int THREADS = 256;          // of a block of the gradient
 constexpr int CANDIDATES = 1024;      // elements at or above the bound that a block can hold; more (ties, hostile rows) take the exact search
+constexpr int AGAIN = 512;            // chunks that may be read again before a row takes the exact search
 constexpr int UNROLL = 4;             // 16-byte vectors a thread of the gradient has in flight
 constexpr int CHUNKS = 16;            // parts of a thread's slice whose maxima are kept
-constexpr int AGAIN = 512;            // chunks that may be read again before a row takes the exact search
 
-template <typename T> struct Traits;
-// BOUND_BITS: leading bits of an order key that the bound of the top list is made from: all that a 16-bit value has; for FP32 a
-// slightly lower bound lets hardly more candidates through and takes fewer steps.
-// LOG_ROUND: log2 of the 16-byte vectors that a thread has in flight (2048 rows of 32000 FP32: 44.2 us at eight, 47.7 at four; 2048 of
-// 128000 BF16, which needs more registers a vector: 95 and 90).
-template <> struct Traits<float> { static constexpr int PER = 4, BOUND_BITS = 24, LOG_ROUND = 3; };
-template <> struct Traits<bf> { static constexpr int PER = 8, BOUND_BITS = 16, LOG_ROUND = 2; };
-template <> struct Traits<__half> { static constexpr int PER = 8, BOUND_BITS = 19, LOG_ROUND = 2; };
+constexpr int LOG_ROUND = 3;          // log2 of the 16-byte vectors a thread of the scores has in flight (2048 x 64000 BF16, 5 alternatives: 52.7 us, at four vectors 57.5)
+constexpr int BOUND_BITS = 16;        // leading bits of an order key that the bound of the top list is made from: a step of 2^-7 lets few more elements through
+
+template <typename T> struct Traits { static constexpr int PER = 16 / sizeof(T); };
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(bf v) { return __bfloat162float(v); }
@@ -92,17 +87,12 @@ __device__ __forceinline__ void move_to(Stats& a, float m) {
     const float d = fmaxf(a.m - m, LEAST), f = ex2(d);
     a.t = f * (a.t + a.s * d); a.s *= f; a.m = m;
 }
-// Two disjoint sets of elements, joined.
-__device__ __forceinline__ Stats join(Stats a, Stats b) {
-    const float m = max_nan(a.m, b.m);
-    move_to(a, m); move_to(b, m);
-    return {m, a.s + b.s, a.t + b.t};
-}
-// Over the lanes of a warp whose numbers differ below `span`.
+// Over the lanes of a warp whose numbers differ below `span` (lanes span apart hold the same): one maximum, one move, then two sums.
 __device__ __forceinline__ Stats join_lanes(Stats st, int span) {
-#pragma unroll 1
-    for (int d = span >> 1; d > 0; d >>= 1)
-        st = join(st, {__shfl_xor_sync(0xffffffffu, st.m, d), __shfl_xor_sync(0xffffffffu, st.s, d), __shfl_xor_sync(0xffffffffu, st.t, d)});
+    move_to(st, value_of((Entry)__reduce_max_sync(0xffffffffu, order_key(st.m)) << 32));
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1)
+        if (d < span) { st.s += __shfl_xor_sync(0xffffffffu, st.s, d); st.t += __shfl_xor_sync(0xffffffffu, st.t, d); }
     return st;
 }
 
@@ -210,26 +200,29 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(const void* at, uint32_t rank
 }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
 
-struct Shared {
+template <int THREADS> struct Shared {
+    static constexpr int WARPS = THREADS / 32;
     Entry entry[CANDIDATES];
     Entry list[RB_MAX_TOP];
     Stats warp[WARPS];
     float most[WARPS];
     Stats mine;                          // this block's part, read by the cluster's first block
     float chunk[CHUNKS][THREADS];        // largest element of each thread's chunks
-    uint16_t again[AGAIN];               // chunks to read again: thread + 256 * chunk
+    uint16_t again[AGAIN];               // chunks to read again: thread + 256 * chunk (at most 256 threads)
     uint32_t all[WARPS], any[WARPS];     // of the slices' keys
     uint32_t found, again_count;
     uint32_t tie_warp[WARPS];
 };
 
-__device__ __forceinline__ void push(Shared& sh, uint32_t key, uint32_t at) {
+template <int THREADS>
+__device__ __forceinline__ void push(Shared<THREADS>& sh, uint32_t key, uint32_t at) {
     const uint32_t i = atomicAdd(&sh.found, 1u);
     if (i < CANDIDATES) sh.entry[i] = entry_of(key, at);
 }
 
 // Candidates -> sorted list of the first `want`.  The number of candidates in front of one is its place; eight lanes count for each.
-__device__ __forceinline__ void rank_candidates(Shared& sh, uint32_t count, uint32_t want) {
+template <int THREADS>
+__device__ __forceinline__ void rank_candidates(Shared<THREADS>& sh, uint32_t count, uint32_t want) {
     const uint32_t part = threadIdx.x & 7;
     for (uint32_t base = 0; base < count; base += THREADS / 8) {
         const uint32_t i = base + (threadIdx.x >> 3);
@@ -244,7 +237,8 @@ __device__ __forceinline__ void rank_candidates(Shared& sh, uint32_t count, uint
 }
 // Sorted lists of k entries, one after the other in sh.entry, into one sorted list of k.  An entry's place is its place in its own list
 // and the number of larger entries in each other one, found by halving.  Empty entries (0) are behind all others and never placed.
-__device__ __forceinline__ void merge_lists(Shared& sh, uint32_t lists, uint32_t k) {
+template <int THREADS>
+__device__ __forceinline__ void merge_lists(Shared<THREADS>& sh, uint32_t lists, uint32_t k) {
     for (uint32_t i = threadIdx.x; i < lists * k; i += THREADS) {
         const uint32_t own = i / k;
         const Entry e = sh.entry[i];
@@ -275,8 +269,8 @@ __device__ __forceinline__ uint32_t kth_of_block(uint32_t key, uint32_t k, uint3
 }
 
 // Elements [first, last) of the row that are > bound (or >=), counted by the whole block.
-template <typename T>
-__device__ uint32_t count_in_block(Shared& sh, const T* row, uint32_t first, uint32_t last, uint32_t bound, bool or_equal) {
+template <typename T, int THREADS>
+__device__ uint32_t count_in_block(Shared<THREADS>& sh, const T* row, uint32_t first, uint32_t last, uint32_t bound, bool or_equal) {
     __syncthreads();
     if (threadIdx.x == 0) sh.found = 0;
     __syncthreads();
@@ -291,13 +285,14 @@ __device__ uint32_t count_in_block(Shared& sh, const T* row, uint32_t first, uin
 // Rows on which the bound lets too many elements through: many equal ones (a masked vocabulary, a constant row) or a hostile order.
 // `bound` is the k-th largest slice maximum itself, so that equal elements are equal to it.  Takes the elements above it, after tightening it to the exact k-th value where they would not fit, then fills up with the
 // equal ones of lowest index.
-template <typename T>
-__device__ __noinline__ void exact_candidates(Shared& sh, const T* row, uint32_t first, uint32_t last, uint32_t bound, uint32_t want) {
-    if (count_in_block<T>(sh, row, first, last, bound, false) > CANDIDATES) {
+template <typename T, int THREADS>
+__device__ __noinline__ void exact_candidates(Shared<THREADS>& sh, const T* row, uint32_t first, uint32_t last, uint32_t bound, uint32_t want) {
+    constexpr int WARPS = THREADS / 32;
+    if (count_in_block<T, THREADS>(sh, row, first, last, bound, false) > CANDIDATES) {
         bound = 0;
         for (int bit = 31; bit >= 0; --bit) {
             const uint32_t trial = bound | (1u << bit);
-            if (count_in_block<T>(sh, row, first, last, trial, true) >= want) bound = trial;
+            if (count_in_block<T, THREADS>(sh, row, first, last, trial, true) >= want) bound = trial;
         }
     }
     __syncthreads();
@@ -330,8 +325,9 @@ __device__ __noinline__ void exact_candidates(Shared& sh, const T* row, uint32_t
 // A whole row by one block, for the rows that the fast form does not answer: nothing but masks, infinities, NaN, scales far from one.
 // The exponent is (x - M) c with M the largest element itself, held at -1000 and above, where a logit of -inf then counts as 0.
 // m of the result is M, not its product with c.
-template <typename T>
-__device__ __noinline__ Stats careful_row(Shared& sh, const T* row, uint32_t vocab, float c) {
+template <typename T, int THREADS>
+__device__ __noinline__ Stats careful_row(Shared<THREADS>& sh, const T* row, uint32_t vocab, float c) {
+    constexpr int WARPS = THREADS / 32;
     float most = -INFINITY;
     for (uint32_t i = threadIdx.x; i < vocab; i += THREADS) most = max_nan(most, to_f32(row[i]));
 #pragma unroll
@@ -355,32 +351,27 @@ __device__ __noinline__ Stats careful_row(Shared& sh, const T* row, uint32_t voc
     return {most, s, t};
 }
 
-// One row per cluster of `parts` blocks (one block where parts is 1), rows in a grid-stride loop.  2048 x 128000 BF16: 90 us = 5.8 TB/s;
-// 2048 x 32000 FP32: 44 us = 6.0 TB/s, with 5 alternatives 56 (each row's search for them is a chain of barriers and one L2 round
-// trip, which the other blocks of the SM hide in part).
-template <typename T>
-__global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArgs a, const uint32_t parts) {
-    constexpr int PER = Traits<T>::PER, ROUND = 1 << Traits<T>::LOG_ROUND;
-    __shared__ Shared sh;
-    const uint32_t tid = threadIdx.x, lane = tid & 31, rank = parts > 1 ? blockIdx.x % parts : 0;
-    const uint64_t clusters = gridDim.x / parts;
+// One row per cluster of 2^log_parts blocks, rows in a grid-stride loop; TOP: with alternatives.  2048 x 128000 BF16: 84 us = 6.2 TB/s; 2048 x
+// 32000 FP32: 41 us = 6.4 TB/s, with 5 alternatives 47 (each row's search for them is a chain of barriers and one L2 round trip, which
+// the other blocks of the SM hide in part).
+template <typename T, int THREADS, bool TOP>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_scores_kernel(const ScoreArgs a, const uint32_t log_parts) {
+    constexpr int PER = Traits<T>::PER, ROUND = 1 << LOG_ROUND, WARPS = THREADS / 32;
+    __shared__ Shared<THREADS> sh;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, rank = blockIdx.x & ((1u << log_parts) - 1);
+    const uint32_t clusters = gridDim.x >> log_parts;
     rb::predecessor_done();
-    for (uint64_t r = blockIdx.x / parts; r < a.rows; r += clusters) {
+    for (uint64_t r = blockIdx.x >> log_parts; r < a.rows; r += clusters) {
         const T* row = static_cast<const T*>(a.logits) + r * a.ld;
         const RowView<T> view(row, a.vocab);
-        const uint32_t v0 = (uint32_t)((uint64_t)view.vectors * rank / parts), v1 = (uint32_t)((uint64_t)view.vectors * (rank + 1) / parts);
+        const uint32_t v0 = (uint32_t)((uint64_t)view.vectors * rank >> log_parts), v1 = (uint32_t)((uint64_t)view.vectors * (rank + 1) >> log_parts);
         // this block's elements are [first, last): its vectors, the elements in front in the first block, those behind in the last
-        const uint32_t first = rank == 0 ? 0 : view.head + v0 * PER, last = rank + 1 == parts ? a.vocab : view.head + v1 * PER;
+        const uint32_t first = rank == 0 ? 0 : view.head + v0 * PER, last = rank + 1 == 1u << log_parts ? a.vocab : view.head + v1 * PER;
         const uint32_t front = view.head + v0 * PER - first, loose = front + (last - (view.head + v1 * PER));
         const uint32_t loose_at = tid < front ? first + tid : view.head + v1 * PER + (tid - front);   // valid for tid < loose
 
-        int64_t id = a.ignore;
-        float chosen = 0.f;
-        if (tid == 0 && rank == 0) {
-            id = a.wide_ids ? static_cast<const int64_t*>(a.ids)[r] : (int64_t) static_cast<const int32_t*>(a.ids)[r];
-            if (id != a.ignore && (id < 0 || id >= (int64_t)a.vocab)) { if (a.bad) atomicExch(a.bad, 1); id = a.ignore; }
-            if (id != a.ignore && id >= 0 && id < (int64_t)a.vocab) chosen = to_f32(row[id]);
-        }
+        int64_t id = a.ignore;      // asked for here, looked at when the row has been read: the first warp does not wait for it
+        if (tid == 0 && rank == 0) id = a.wide_ids ? static_cast<const int64_t*>(a.ids)[r] : (int64_t) static_cast<const int32_t*>(a.ids)[r];
 
         Running run{a.start, 0.f, 0.f, 0.f, 0.f, -INFINITY};
         const Vec<T>* vec = view.vec();
@@ -391,9 +382,11 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
         uint32_t v = v0 + tid, round = 0;
         float chunk_top = -INFINITY;
         auto note = [&](float top) {
-            chunk_top = max_nan(chunk_top, top);
-            if (a.k) sh.chunk[round >> chunk_shift][tid] = chunk_top;
-            if ((++round & ((1u << chunk_shift) - 1)) == 0) chunk_top = -INFINITY;
+            if constexpr (TOP) {
+                chunk_top = max_nan(chunk_top, top);
+                sh.chunk[round >> chunk_shift][tid] = chunk_top;
+                if ((++round & ((1u << chunk_shift) - 1)) == 0) chunk_top = -INFINITY;
+            }
         };
         for (; v + (ROUND - 1) * THREADS < v1; v += THREADS * ROUND) {
             Vec<T> got[ROUND];
@@ -412,11 +405,16 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
             got[0].v[0] = row[loose_at];
             take<T, 1>(run, got, a);
         }
+        float chosen = 0.f;
+        if (tid == 0 && rank == 0) {
+            if (id != a.ignore && (id < 0 || id >= (int64_t)a.vocab)) { if (a.bad) atomicExch(a.bad, 1); id = a.ignore; }
+            if (id != a.ignore && id >= 0 && id < (int64_t)a.vocab) chosen = to_f32(row[id]);
+        }
         const uint32_t slice_key = order_key(run.most);
 
         Stats st = join_lanes({run.m, run.s0 + run.s1, run.t0 + run.t1}, 32);
         if (lane == 0) sh.warp[tid >> 5] = st;
-        if (a.k) {
+        if constexpr (TOP) {
             const uint32_t all = __reduce_and_sync(0xffffffffu, slice_key), any = __reduce_or_sync(0xffffffffu, slice_key);
             if (lane == 0) { sh.all[tid >> 5] = all; sh.any[tid >> 5] = any; }
         }
@@ -425,10 +423,10 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
         if (tid < 32) st = join_lanes(sh.warp[lane % WARPS], WARPS);
 
         uint32_t want = 0;
-        if (a.k) {
+        if constexpr (TOP) {
             want = a.k < last - first ? a.k : last - first;
             const uint32_t all = __reduce_and_sync(0xffffffffu, sh.all[lane % WARPS]), any = __reduce_or_sync(0xffffffffu, sh.any[lane % WARPS]);
-            const uint32_t bound = kth_of_block<Traits<T>::BOUND_BITS>(slice_key, a.k, all, any);
+            const uint32_t bound = kth_of_block<BOUND_BITS>(slice_key, a.k, all, any);
             if (slice_key >= bound) {
                 const uint32_t mine = (round + (1u << chunk_shift) - 1) >> chunk_shift;
                 for (uint32_t c = 0; c < mine; ++c)
@@ -438,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
             __syncthreads();
             const uint32_t again = sh.again_count;
             if (again <= AGAIN) {
-                const uint32_t per = Traits<T>::LOG_ROUND + chunk_shift;        // log2 of a chunk's vectors
+                const uint32_t per = LOG_ROUND + chunk_shift;        // log2 of a chunk's vectors
                 for (uint32_t i = tid; i < again << per; i += THREADS) {
                     const uint32_t which = sh.again[i >> per], at = v0 + (which & 255) + ((which >> 8 << per) + (i & ((1u << per) - 1))) * THREADS;
                     if (at < v1) {
@@ -455,12 +453,13 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
                 }
             }
             __syncthreads();
-            if (again > AGAIN || sh.found > CANDIDATES) exact_candidates<T>(sh, row, first, last, kth_of_block<32>(slice_key, a.k, all, any), want);
+            if (again > AGAIN || sh.found > CANDIDATES) exact_candidates<T, THREADS>(sh, row, first, last, kth_of_block<32>(slice_key, a.k, all, any), want);
             rank_candidates(sh, sh.found, want);
         }
-        if (parts > 1) {
+        if (log_parts) {
+            const uint32_t parts = 1u << log_parts;
             if (tid == 0) sh.mine = st;
-            if (tid >= want && tid < a.k) sh.list[tid] = 0;      // fewer elements than entries
+            if (TOP && tid >= want && tid < a.k) sh.list[tid] = 0;      // fewer elements than entries
             cluster_sync();
             if (rank == 0) {
                 // one part per lane of the first warp; one list entry per thread
@@ -469,7 +468,7 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
                     st = join_lanes({__uint_as_float(ld_cluster_u32(&sh.mine.m, from)), __uint_as_float(ld_cluster_u32(&sh.mine.s, from)),
                                      __uint_as_float(ld_cluster_u32(&sh.mine.t, from))}, (int)parts);
                 }
-                if (a.k) {
+                if constexpr (TOP) {
                     for (uint32_t i = tid; i < parts * a.k; i += THREADS) sh.entry[i] = ld_cluster_u64(&sh.list[i % a.k], i / a.k);
                     __syncthreads();
                     merge_lists(sh, parts, a.k);
@@ -484,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
             const bool fast = !a.careful && st.m > a.start && fabsf(st.m) < 1048576.0f;      // beyond 2^20 the rounding of m itself would be felt in d
             float reference, logs;               // log p of x is ln2 (c x - reference) - logs, or scale (x - reference) - logs
             if (fast) { reference = st.m; logs = LN2 * log2f(st.s); }
-            else { st = careful_row<T>(sh, row, a.vocab, a.c); reference = st.m; logs = logf(st.s); }
+            else { st = careful_row<T, THREADS>(sh, row, a.vocab, a.c); reference = st.m; logs = logf(st.s); }
             const float lse = fast ? fmaf(LN2, reference, logs) : fmaf(reference, a.scale, logs);
             auto log_p = [&](float x) {
                 if (!fast) return fmaf(x - reference, a.scale, -logs);
@@ -495,13 +494,13 @@ __global__ void __launch_bounds__(THREADS, 4) token_scores_kernel(const ScoreArg
                 a.log_probs[r] = id == a.ignore ? 0.f : log_p(chosen);
                 if (a.entropy) { const float h = logs - LN2 * (st.t / st.s); a.entropy[r] = h < 0.f ? 0.f : h; }
             }
-            if (tid < a.k) {
+            if (TOP && tid < a.k) {
                 const Entry e = sh.list[tid];
                 a.top_ids[r * a.k + tid] = (int32_t)index_of(e);
                 a.top_values[r * a.k + tid] = log_p(value_of(e));
             }
         }
-        if (parts > 1) cluster_sync();       // the lists of this row have been read
+        if (log_parts) cluster_sync();       // the lists of this row have been read
         else __syncthreads();
     }
 }
@@ -621,22 +620,37 @@ __global__ void __launch_bounds__(THREADS, 5) token_scores_grad_kernel(const Gra
 
 bool is_float(uint32_t dtype) { return dtype == RB_F32 || dtype == RB_BF16 || dtype == RB_F16; }
 
-template <typename T>
+template <typename T, int THREADS, bool TOP>
 void launch_scores(rb_ctx* ctx, const ScoreArgs& a) {
-    // A row is one block's work where the rows fill the GPU or are short; few long rows are split over clusters of two or four blocks.
-    // us for 4 rows at 1 / 2 / 4 / 8 blocks a row: 128000 BF16, 20 alternatives 15.4 / 12.7 / 10.8 / 11.0; 32000 BF16 8.1 / 8.9 / 9.0 / 10.0
-    // (the join of the lists costs what the split saves); for 148 rows of 128000: 22.6 / 18.4 / 27.7 / 49.
     static rb::OncePerDevice once;
-    const cudaError_t counted = once.run(ctx, [](int& blocks) { return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, token_scores_kernel<T>, THREADS, 0); });
+    const cudaError_t counted = once.run(ctx, [](int& blocks) { return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, token_scores_kernel<T, THREADS, TOP>, THREADS, 0); });
     const int resident = counted == cudaSuccess && once.value[ctx->device] > 0 ? once.value[ctx->device] : 1;
     const uint64_t slots = (uint64_t)ctx->sm_count * resident, bytes = (uint64_t)a.vocab * sizeof(T);
-    uint32_t parts = 1;
-    if (bytes >= (a.k ? 160u : 96u) * 1024)
-        while (parts < 4 && a.rows * parts * 2 <= 3ull * ctx->sm_count) parts *= 2;
+    // A row is one block's work where the rows fill the GPU or are short; few long rows are split over clusters.  us at 1 / 2 / 4 / 8 blocks
+    // a row: 4 x 128000 BF16 with 20 alternatives 14.6 / 11.9 / 8.9 / 9.5, without 5.0 / 4.3 at 4 / 8; 4 x 32000 BF16 with 20 6.2 / 7.8 (the join
+    // of the lists costs what the split saves).
+    uint32_t log_parts = 0;
+    if (bytes >= (TOP ? 160u : 96u) * 1024)
+        while (log_parts < (TOP ? 2 : 3) && a.rows << (log_parts + 1) <= 3ull * ctx->sm_count) ++log_parts;
+    const uint32_t parts = 1u << log_parts;
     const uint64_t clusters = a.rows < slots / parts ? a.rows : slots / parts;
     // Blocks that take several rows keep the placement of an empty GPU, which spreads the longer lists over the SMs (2048 rows of 128000
     // BF16: 90 us, overlapped 107).
-    rb::launch_behind(ctx, token_scores_kernel<T>, clusters * parts, THREADS, 0, parts, a.rows <= clusters, a, parts);
+    rb::launch_behind(ctx, token_scores_kernel<T, THREADS, TOP>, clusters * parts, THREADS, 0, parts, a.rows <= clusters, a, log_parts);
+}
+
+template <typename T>
+void launch_scores(rb_ctx* ctx, const ScoreArgs& a) {
+    // Blocks start together and so reach the search for the alternatives together, with DRAM idle meanwhile: with many rows, twice the rows
+    // at a time in half the threads each meet it half as often.
+    // us at 128 / 256 threads: 8000 rows of 4000 BF16, 5 alternatives 48 / 89, without 28 / 46; 2048 of 32000 FP32, 5: 48.6 / 51.3, 60: 65.8 /
+    // 61.9; 2048 of 128000 BF16, 5: 102 / 107, without 94 / 91; 500 of 32003 FP32, 5: 20 / 16.
+    const bool many = a.rows > 4ull * ctx->sm_count, shorter = (uint64_t)a.vocab * sizeof(T) <= 64 * 1024;
+    if (a.k == 0) {
+        if (many && shorter) launch_scores<T, 128, false>(ctx, a);
+        else launch_scores<T, 256, false>(ctx, a);
+    } else if (many && (shorter || a.k <= 32)) launch_scores<T, 128, true>(ctx, a);
+    else launch_scores<T, 256, true>(ctx, a);
 }
 
 }  // namespace

@@ -24,9 +24,9 @@ def compare(got, want, vocab, top):
     log_prob, lse, entropy, values, ids = got
     w_log_prob, w_lse, w_entropy, w_values, w_ids, _ = want
     d = spread(vocab)
-    with np.errstate(invalid="ignore"):
+    with np.errstate(invalid="ignore", over="ignore"):
         for a, w, extra in ((log_prob, w_log_prob, 0), (lse, w_lse, 0), (entropy, w_entropy, 20 * d)) + (((values, w_values, 0),) if top else ()):
-            same = (np.isnan(a) & np.isnan(w)) | (a == w)
+            same = (np.isnan(a) & np.isnan(w)) | (a == w) | (np.isinf(a) & (a == w.astype(np.float32)))      # beyond FP32's range the rounded result is infinite
             off = np.where(same, 0, np.abs(a - w) - (d + extra + 6 * U * np.abs(w)))
             assert off.max(initial=0) <= 0, off.max()
     if top:
@@ -123,6 +123,30 @@ def test_outputs_may_be_left_out_and_neighbours_stay(client):
     RT.token_log_probs(client, t, i, out=out)
     for a, b in zip(full[:2], out):
         assert np.array_equal(client.read(a), client.read(b))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("vocab,top,pad", [(70, 0, 0), (70, 7, 3), (70, 64, 0), (3001, 1, 0), (3001, 32, 1), (3001, 33, 0), (3001, 64, 5), (9000, 5, 8), (34000, 0, 0), (34000, 20, 1)])
+def test_many_rows(client, dtype, vocab, top, pad):
+    """More rows than blocks of the larger kind fit the GPU, ordinary ones among masked, constant, tied, ascending and special ones."""
+    rows = 700 if vocab < 30000 else 610
+    rng, x, _, ids = case(rows, vocab + pad, dtype, seed=3)
+    rows_of = lambda n: slice(n, None, 40)
+    low = {F32: np.float32(np.finfo(np.float32).min), BF16: np.uint16(0xff7f), F16: np.float16(-65504)}[dtype]
+    inf, nan = {F32: (np.float32(np.inf), np.float32(np.nan)), BF16: (np.uint16(0x7f80), np.uint16(0x7fc0)), F16: (np.float16(np.inf), np.float16(np.nan))}[dtype]
+    minus = np.uint16(0xff80) if dtype == BF16 else -inf
+    x[rows_of(1), vocab // 2:] = minus
+    x[rows_of(2), vocab // 3:] = low
+    x[rows_of(3)] = x[3, 0]
+    x[rows_of(4)] = minus
+    x[rows_of(5), 5] = nan
+    x[rows_of(6), 9] = inf
+    x[rows_of(7)] = np.sort(x[rows_of(7)] if dtype != BF16 else x[rows_of(7)] & 0x7fff)
+    x[rows_of(8), ::2] = x[8, 0]
+    values = {F32: lambda a: a, F16: lambda a: a.astype(np.float32), BF16: R.bf16_bits_to_f32}[dtype](x)[:, :vocab]
+    t = client.upload(x, dtype)
+    view = TensorBuffer(t.handle, (rows, vocab), dtype, (vocab + pad, 1), 0, t._owner)
+    call(client, None, values, np.where(ids >= vocab, 0, ids), dtype, 1.25, top, view=view)
 
 
 # ---- gradient --------------------------------------------------------------------------------------------------------------------
