@@ -227,7 +227,7 @@ __device__ __forceinline__ Factor factor_of(const QuantArgs& a, uint64_t row, ui
 // wait for each other).  Everything that the threads of a row compute alike is kept to one division: the root and the scale are the
 // first thread's business.
 template <typename T, typename TW, int MODE, int VEC, int UNROLL>
-__global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
+__global__ void __launch_bounds__(512, MODE == PLAIN ? 3 : 2) quant_rows_kernel(const QuantArgs a) {
     constexpr bool NORMS = MODE == NORM || MODE == ADD_NORM, TWO = MODE == GATED || MODE == ADD_NORM;
     typedef typename std::conditional<MODE == GATED, float, T>::type H;
     typedef Held<H, VEC> Hold;
@@ -255,15 +255,17 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
                 const uint32_t i = base + u * threads;
-                const uint32_t at = decltype(whole)::value || i < vectors ? i : vectors - 1;      // behind the row: the last vector again, not used
+                const uint32_t at = decltype(whole)::value || i < vectors ? i : base;      // behind the row: the thread's first vector of the round once more
                 if (NORMS) wt[NORMS ? u : 0] = weight[at];
                 in[u] = x[at];
                 if (TWO) in2[TWO ? u : 0] = o[at];
             }
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
-                const uint32_t i = base + u * threads;
-                if (!decltype(whole)::value && i >= vectors) break;
+                // No branch on it: that would move the loads down to where they are used, one DRAM latency after the other (8000 x 5000 FP32: 58 us
+                // instead of 37).  What is done twice gives the same again, except for the sum.
+                const bool live = decltype(whole)::value || base + u * threads < vectors;
+                const uint32_t i = live ? base + u * threads : base;
                 float v[VEC];
                 [[maybe_unused]] float w[VEC];
                 if constexpr (MODE == ADD_NORM) { in[u] = sum_of<T, VEC>(in[u], in2[u]); xo[i] = in[u]; }
@@ -271,11 +273,13 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
                 if constexpr (MODE == GATED) { widen<T, VEC>(in2[u], w); silu_mul<VEC>(v, w); if (i < a.held) Hold::put(mine, a.held, i, narrow<float, VEC>(v)); }
                 else if (i < a.held) Hold::put(mine, a.held, i, in[u]);
                 if constexpr (NORMS) {
+                    const float old0 = sum0, old1 = sum1;
                     if constexpr (VEC % 2 != 0) sum0 = __fmaf_rn(v[0], v[0], sum0);
                     else {
 #pragma unroll
                         for (int j = 0; j < VEC; j += 2) fma2(sum0, sum1, v[j], v[j + 1], v[j], v[j + 1]);
                     }
+                    if (!live) { sum0 = old0; sum1 = old1; }
                     widen<TW, VEC>(wt[u], w);
                     times<VEC>(v, w);
                 }
@@ -287,8 +291,12 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
             }
         };
         uint32_t base = tid;
-        for (; base + (UNROLL - 1) * threads < vectors; base += UNROLL * threads) chunk(base, std::true_type());
-        if (base < vectors) chunk(base, std::false_type());
+        // The norm's full rounds without the selections, for whole warps (base | 31 is the last lane): a warp that went both ways would wait for
+        // DRAM twice.
+        if constexpr (NORMS) {
+            for (; (base | 31) + (UNROLL - 1) * threads < vectors; base += UNROLL * threads) chunk(base, std::true_type());
+            if (base < vectors) chunk(base, std::false_type());
+        } else for (; base < vectors; base += UNROLL * threads) chunk(base, std::false_type());
 
         constexpr int AHEAD = NORMS && sizeof(Weight) > 16 ? 2 : 4;
         // magnitudes compare as integers, and in that order NaN lies above infinity
@@ -346,11 +354,11 @@ __global__ void __launch_bounds__(512, 2) quant_rows_kernel(const QuantArgs a) {
     }
 }
 
-// Plain rows that start anywhere (an odd width): vectors from the row's first 16-byte boundary on, the elements around them one by
+// Plain rows that start anywhere (an odd width; 4000 x 14335 BF16: 38 us, aligned 30): vectors from the row's first 16-byte boundary on, the elements around them one by
 // one, and single bytes out.  The row lies in shared memory with its vectors aligned, so element e is at e + VEC - head, and is read
 // back by other threads than wrote it: lanes on neighbouring elements.
 template <typename T>
-__global__ void __launch_bounds__(512, 2) quant_shifted_kernel(const QuantArgs a) {
+__global__ void __launch_bounds__(512, 3) quant_shifted_kernel(const QuantArgs a) {
     constexpr int VEC = 16 / sizeof(T), UNROLL = 4;
     typedef Pack<T, VEC> In;
     extern __shared__ __align__(16) uint8_t s_rows[];
@@ -405,7 +413,7 @@ __global__ void __launch_bounds__(512, 2) quant_shifted_kernel(const QuantArgs a
     }
 }
 
-constexpr uint32_t SHIFTED_VECTORS = 4;      // 1777 x 5003 FP32: 11.8 us at four vectors a thread, 12.1 at eight, 14.4 at twelve (single elements throughout: 16.0)
+constexpr uint32_t SHIFTED_VECTORS = 4;      // 1777 x 5003 FP32: 10.9 us at four vectors a thread; at eight 3 % more, at twelve 22 % (single elements throughout: 16.0)
 constexpr uint32_t ROW_SMEM = 96 * 1024;     // shared memory a row may take: at least two rows an SM
 
 template <typename T, typename TW, int MODE, int VEC, int UNROLL>

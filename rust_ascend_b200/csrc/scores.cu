@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_scores_kernel(c
                 if ((++round & ((1u << chunk_shift) - 1)) == 0) chunk_top = -INFINITY;
             }
         };
-        for (; v + (ROUND - 1) * THREADS < v1; v += THREADS * ROUND) {
+        for (; v - lane + 31 + (ROUND - 1) * THREADS < v1; v += THREADS * ROUND) {      // whole warps: none waits for DRAM once on either side
             Vec<T> got[ROUND];
 #pragma unroll
             for (int u = 0; u < ROUND; ++u) got[u] = vec[v + u * THREADS];

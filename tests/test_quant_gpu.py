@@ -253,3 +253,61 @@ def test_more_than_2_to_the_32_values(client):
     client.read_into(x.handle, back, (rows - 1) * width * 2)
     with np.errstate(over="ignore"):
         assert np.array_equal(back, (b.astype(np.float32) @ a[-1].astype(np.float32)).astype(np.float16))
+
+
+@pytest.mark.parametrize("width", [256, 301, 1000, 5003, 8192, 8193, 12000, 16384, 16390])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_silu_rows_that_start_anywhere(client, width, dtype):
+    """Gate and up at any element of wider rows, each at another distance from a 16-byte boundary: what aligned rows give, bit for bit."""
+    rng = np.random.default_rng([width, int(dtype)])
+    rows = 7
+    gate, gv = R.hold(np.clip(rng.standard_normal((rows, width)) * 2, -6.5, 6.5), dtype)
+    up, uv = R.hold(np.clip(rng.standard_normal((rows, width)) * 2, -6.5, 6.5), dtype)
+    per = 16 // dtype.size
+    wanted = R.silu_mul(gv, uv)
+    first = None
+    for at, far in ((0, 0), (1, 0), (0, per - 1), (3, 2), (per - 1, 1)):
+        pitch = (2 * width + 64) // per * per + (per + 1 if at % 2 else 0)
+        wide = np.zeros((rows, pitch), gate.dtype)
+        second = (width + 2 * per) // per * per + far
+        wide[:, at:at + width], wide[:, second:second + width] = gate, up
+        t = client.upload(wide, dtype)
+        view = lambda start: TensorBuffer(t.handle, (rows, width), dtype, (pitch, 1), start * dtype.size, t._owner)
+        q, s = RT.quantize_rows(client, view(at), up=view(second))
+        got = client.read(q), client.read(s)
+        R.check_rows(*got, wanted, SILU + 2 * 2.0 ** -24, SILU + VALUE)
+        first = first or got
+        assert np.array_equal(got[0], first[0]) and np.array_equal(got[1], first[1])
+        assert np.array_equal(client.read(t), wide)
+
+
+@pytest.mark.parametrize("width", [303, 5001, 9001])
+def test_special_values_in_silu_rows_that_start_anywhere(client, width):
+    rng = np.random.default_rng(width)
+    g, u = rng.standard_normal((7, width)).astype(np.float32), rng.standard_normal((7, width)).astype(np.float32)
+    g[1, 2], u[2, width - 1], g[3, width // 2] = np.nan, np.inf, np.inf
+    g[4], u[5] = 0, 0
+    u[6] *= 1e-30                                         # values that are raised before they are divided
+    q, s = (client.read(t) for t in RT.quantize_rows(client, client.upload(g), up=client.upload(u)))
+    assert np.isnan(s[1:4]).all() and not q[1:6].any() and np.all(s[4:6] == np.float32(2.0 ** -126))
+    R.check_rows(q[[0, 6]], s[[0, 6]], R.silu_mul(g[[0, 6]], u[[0, 6]]), SILU + 2 * 2.0 ** -24, SILU + VALUE)
+
+
+@pytest.mark.parametrize("rows,width", [(3, 4), (9, 1032), (170, 5000), (300, 2056), (5, 20008), (160, 1004)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_rows_that_end_inside_a_round(client, rows, width, dtype, residual):
+    """Widths whose last vectors fill only some lanes of a warp, with the sum written over the input."""
+    rng = np.random.default_rng([rows, width, int(dtype), residual])
+    x, xv = R.hold(rng.standard_normal((rows, width)), dtype)
+    d, dv = R.hold(rng.standard_normal((rows, width)), dtype)
+    w, wv = R.hold(1 + 0.2 * rng.standard_normal(width), dtype)
+    t, wt = client.upload(x, dtype), client.upload(w, dtype)
+    total = xv
+    if residual:
+        total = R.hold(xv + dv, dtype)[1]
+        q, s, stored = RT.rms_norm_quant(client, t, wt, 1e-5, delta=client.upload(d, dtype), out=(None, None, t))
+        assert np.array_equal(R.read(client, stored), total)
+    else:
+        q, s = RT.rms_norm_quant(client, t, wt, 1e-5)
+    R.check_rows(client.read(q), client.read(s), R.norm(total, wv, 1e-5), NORM_SCALE, VALUE)
