@@ -34,7 +34,9 @@ constexpr int UNROLL = 4;             // 16-byte vectors a thread of the gradien
 constexpr int CHUNKS = 16;            // parts of a thread's slice whose maxima are kept
 
 constexpr int LOG_ROUND = 3;          // log2 of the 16-byte vectors a thread of the scores has in flight (2048 x 64000 BF16, 5 alternatives: 52.7 us, at four vectors 57.5)
-constexpr int BOUND_BITS = 16;        // leading bits of an order key that the bound of the top list is made from: a step of 2^-7 lets few more elements through
+// Where the search for the bound of the top list ends: a step of 2^-7 of a value lets few more elements through (2048 x 32000 FP32: 54 us, with
+// eight more bits 56), rows that lie closer together take eight steps all the same.
+constexpr int LEAST_BIT = 16, BOUND_STEPS = 8;
 
 template <typename T> struct Traits { static constexpr int PER = 16 / sizeof(T); };
 
@@ -253,15 +255,15 @@ __device__ __forceinline__ void merge_lists(Shared<THREADS>& sh, uint32_t lists,
     }
 }
 
-// The largest bound of BITS leading bits that k of the block's keys (one per thread) reach, bit by bit from the first in which the
-// keys differ; `all` and `any` are their conjunction and disjunction.
-template <int BITS>
+// The largest bound that k of the block's keys (one per thread) reach, bit by bit from the first in which the keys differ, down to the last
+// one (EXACT) or to LEAST_BIT, but at least BOUND_STEPS of them; `all` and `any` are their conjunction and disjunction.
+template <bool EXACT>
 __device__ __forceinline__ uint32_t kth_of_block(uint32_t key, uint32_t k, uint32_t all, uint32_t any) {
     const int top = 31 - __clz((int)(all ^ any));             // -1: all alike
     uint32_t bound = top < 0 ? any : any & ~(0xffffffffu >> (31 - top));
-    if (top < 0) bound &= ~(0xffffffffu >> (BITS - 1) >> 1);
+    const int least = EXACT ? 0 : max(0, min(LEAST_BIT, top + 1 - BOUND_STEPS));
 #pragma unroll 1
-    for (int bit = top; bit >= 32 - BITS; --bit) {
+    for (int bit = top; bit >= least; --bit) {
         const uint32_t trial = bound | (1u << bit);
         if ((uint32_t)__syncthreads_count(key >= trial) >= k) bound = trial;
     }
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_scores_kernel(c
         if constexpr (TOP) {
             want = a.k < last - first ? a.k : last - first;
             const uint32_t all = __reduce_and_sync(0xffffffffu, sh.all[lane % WARPS]), any = __reduce_or_sync(0xffffffffu, sh.any[lane % WARPS]);
-            const uint32_t bound = kth_of_block<BOUND_BITS>(slice_key, a.k, all, any);
+            const uint32_t bound = kth_of_block<false>(slice_key, a.k, all, any);
             if (slice_key >= bound) {
                 const uint32_t mine = (round + (1u << chunk_shift) - 1) >> chunk_shift;
                 for (uint32_t c = 0; c < mine; ++c)
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_scores_kernel(c
                 }
             }
             __syncthreads();
-            if (again > AGAIN || sh.found > CANDIDATES) exact_candidates<T, THREADS>(sh, row, first, last, kth_of_block<32>(slice_key, a.k, all, any), want);
+            if (again > AGAIN || sh.found > CANDIDATES) exact_candidates<T, THREADS>(sh, row, first, last, kth_of_block<true>(slice_key, a.k, all, any), want);
             rank_candidates(sh, sh.found, want);
         }
         if (log_parts) {

@@ -108,6 +108,15 @@ def test_hostile_order_for_the_top_list(client):
     call(client, x, xv, ids, BF16, 1.0, 17)
 
 
+@pytest.mark.parametrize("rows,vocab", [(3, 30000), (640, 5000)])
+@pytest.mark.parametrize("offset,width", [(1000.0, 0.5), (-300.0, 0.01), (64.0, 1e-4), (1.9, 0.3), (0.0, 1e-30)])
+def test_logits_close_together(client, rows, vocab, offset, width):
+    """Rows whose largest values share many leading bits, and rows around a power of two."""
+    rng = np.random.default_rng([rows, int(width * 1e4)])
+    x = (offset + rng.standard_normal((rows, vocab)) * width).astype(np.float32)
+    call(client, x, x, rng.integers(0, vocab, rows), F32, 1.0, 20)
+
+
 def test_ids_outside_the_vocabulary_and_other_ignore_index(client):
     rng, x, xv, ids = case(8, 300, F32)
     ids[:4] = (300, -1, 2**40, 7)
