@@ -428,6 +428,7 @@ int32_t launch(rb_ctx* ctx, QuantArgs a, const char* what) {
     // SiLU over 4096 x 14336 BF16: 53.9 us at eight, 57.3 at four.  Few rows: latency, so one vector a thread where that fits.
     const uint32_t wanted = a.rows <= (uint64_t)ctx->sm_count ? 1 : (VEC == 1 ? 20 : (MODE == GATED ? 8 : 4));
     uint32_t warps = (vectors + wanted * 32 - 1) / (wanted * 32);
+    if (warps == 2 && vectors <= wanted * 40) warps = 1;      // a little more than a warp's share: rows of one warp come eight a block (8000 x 516 BF16: 6.1 us, 8.9)
     if (warps > 16) warps = 16;
     a.warps = warps;
     const uint32_t groups = warps == 1 ? 8 : 1;
@@ -452,7 +453,8 @@ int32_t launch_shifted(rb_ctx* ctx, const QuantArgs& a, const char* what) {
     return rb::after_launch(ctx, what);
 }
 
-// The widest vectors on which every row of every operand starts: 16 bytes, 8 bytes, or single elements.
+// The widest vectors on which every row of every operand starts: 16 bytes, 8 bytes, or single elements.  Plain rows that do not start on 16
+// bytes are read as shifted ones, unless they are short (us shifted / 8 bytes or single ones: 8000 x 5004 BF16 26 / 34, 8000 x 301 8.7 / 5.5).
 template <typename T, typename TW, int MODE>
 int32_t dispatch(rb_ctx* ctx, const QuantArgs& a, const char* what) {
     constexpr int FULL = 16 / sizeof(T), HALF = FULL / 2;
@@ -463,8 +465,8 @@ int32_t dispatch(rb_ctx* ctx, const QuantArgs& a, const char* what) {
                on(a.x_out, a.width, sizeof(T), b) && on(a.q, a.width, 1, vec);
     };
     if (fits(FULL)) return launch<T, TW, MODE, FULL, MODE == ADD_NORM ? 2 : 4>(ctx, a, what);
+    if (MODE == PLAIN && a.width >= 700 && a.width * sizeof(T) + 48 <= ROW_SMEM) return launch_shifted<T>(ctx, a, what);
     if (fits(HALF)) return launch<T, TW, MODE, HALF, 4>(ctx, a, what);
-    if (MODE == PLAIN && a.width >= 256 && a.width * sizeof(T) + 48 <= ROW_SMEM) return launch_shifted<T>(ctx, a, what);
     return launch<T, TW, MODE, 1, 4>(ctx, a, what);
 }
 
