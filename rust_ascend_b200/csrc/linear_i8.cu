@@ -523,25 +523,46 @@ int32_t launch(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, uint3
     }
 }
 
-// Which kernel, by the sizes alone.  Figures: us on one B200, weights from DRAM, BF16 result.
-Plan plan_of(const LinearParams& p, uint32_t sms, uint32_t pairs) {
-    auto tiles = [&](uint32_t rows, uint32_t tokens) { return (uint64_t)((p.n + rows - 1) / rows) * ((p.m + tokens - 1) / tokens); };
-    auto share = [&](uint64_t ctas, uint64_t t) { uint64_t s = ctas / t; s = s < 8 ? s : 8; s = s < p.num_kb ? s : p.num_kb; return (uint32_t)(s ? s : 1); };
-    // One or two tokens, and up to four over short rows: no tensor core, no set-up (6144 x 4096: 5.9 / 6.7 / 6.9 for 1 / 2 / 4 tokens against
-    // 8.3; 4096 x 14336: 10.9 / 12.1 / 14.4 against 13.6).
-    if (p.m <= 2 || (p.m <= 4 && p.num_kb < 96)) return {0, 0};
-    // Up to 32 tokens the weights' bytes are everything: one CTA per SM streams them (4096 x 4096, 17 tokens: 7.9 with 4 parts, 9.3 with 2,
-    // 8.5 with 8; 14336 x 4096: 14.1 unsplit, 15.5 with 2).
-    if (p.m <= 32) { const uint32_t t = p.m <= 16 ? 16 : 32; return {t, share(sms, tiles(ROWS, t))}; }
-    // Up to 64 the products and the join weigh more, and two CTAs an SM hide them (6144 x 4096, 64 tokens: 10.9 with 4 parts, 12.0 with 3).
-    if (p.m <= 64) return {64, share(sms * 4 / 3, tiles(ROWS, 64))};
-    // Few tiles: K split four ways or more beats pairs, which cannot split it (4096 x 14336, 128 tokens: 17.7 against 26; 4096 x 4096: 10.8
-    // both), above 128 tokens only for long K (256 tokens, K 14336: 21.8 against 26.3; K 4096: 13.2 against 11.4).
-    const uint32_t few = p.m <= 128 ? 64 : 128, parts = share(2 * sms, tiles(ROWS, few));
-    if (p.m <= 256 && parts >= 4 && (p.m <= 128 || p.num_kb >= 64)) return {few, parts};
-    // Pairs: 256 tokens a tile read the least from L2 and draw the least power (4096 x 14336 x 4096 sustained: 175, 128 tokens: 214);
-    // narrower ones where those would leave half of the pairs idle.
-    return {tiles(2 * ROWS, 256) * 2 <= pairs ? 128u : 256u, 0};
+// Which kernel, by the sizes alone: the least of estimated times in us.  The constants were fitted to 4774 sizes of 3 to 700 tokens (random ones
+// and layers of 1024 to 28672 outputs), each timed with every tile and split; what is chosen takes 1.02 to 1.03 of the best one's time
+// on average, 1.12 in nine of ten cases, where borders in tokens and K took 1.22 and 1.11 on average.  The terms are the kernels' own:
+//   * few tokens: a start; the stages of a CTA's part of K, each at its latency or, where two CTAs share an SM, at the rate of the SM's
+//     port to L2 (rows that do not start on cache lines pass it slower), at least the weights' way out of DRAM; the stores; the join
+//     of the parts; a further wave, which clusters reach earlier because they do not fill every SM.
+//   * pairs: a start and the rounds of tiles.
+Plan plan_of(const LinearParams& p, uint32_t k, uint32_t sms, uint32_t pairs) {
+    // One or two tokens, and up to four over short rows: no tensor core, no set-up (one token, 6144 x 4096: 5.9 us against 7.8; four tokens: K of
+    // 1536 0.85 to 1.09 of the tiles' time, K of 4096 1.1 to 1.2).
+    if (p.m <= 2 || (p.m <= 4 && p.num_kb < 24)) return {0, 0};
+    auto up = [](uint64_t a, uint64_t b) { return (a + b - 1) / b; };
+    auto larger = [](double a, double b) { return a > b ? a : b; };
+    const bool aligned = k % BK == 0;
+    const double weights = (double)p.n * k * 1e-6;
+    Plan best{256, 0};
+    double least = 1e300;
+    auto offer = [&](uint32_t tokens, uint32_t parts, double us) { if (us < least) { least = us; best = {tokens, parts}; } };
+    for (uint32_t tokens = 16; tokens <= 128 && (tokens == 16 || tokens < 2 * p.m); tokens *= 2) {
+        const double used = p.m < tokens ? p.m : tokens;
+        const double latency = 0.195 + 0.0009 * tokens, port = 0.0009 * (ROWS + tokens) * (aligned ? 1.0 : 1.37);
+        for (uint32_t parts = 1; parts <= 8 && parts <= p.num_kb; parts *= 2) {
+            const uint64_t ctas = up(p.n, ROWS) * up(p.m, tokens) * parts;
+            const uint32_t spare = sms > 32 ? sms : 33;
+            const uint32_t seats = parts < 4 ? sms : parts == 4 ? spare - 8 : spare * 13 / 16, wave = parts < 4 ? 2 * sms : parts == 4 ? 2 * spare - 32 : seats;
+            const uint64_t share = up(ctas, seats);      // CTAs of the fullest SM
+            const double body = up(p.num_kb, parts) * ((double)(share / 2) * larger(latency, 2 * port) + (double)(share % 2) * larger(latency, port)) + 0.0125 * used * share / parts;
+            offer(tokens, parts, 1.85 + 1.4 * (double)(up(ctas, wave) - 1) + larger(body, weights / 5.1) + (parts > 1 ? 0.78 + 0.031 * used : 0.0));
+        }
+    }
+    if (p.m > 16) {
+        for (uint32_t tokens = 128; tokens <= 256; tokens *= 2) {
+            const uint64_t tiles = up(p.n, 2 * ROWS) * up(p.m, tokens), rest = tiles % pairs;
+            const double halves = tiles < pairs ? 0.72 : 0.63;      // a short last round runs as half tiles, partly under the round in front
+            const double rounds = (double)(tiles / pairs) + (rest == 0 ? 0.0 : 2 * rest <= pairs ? halves : 1.0);
+            const double tile = p.num_kb * (0.150 + 0.0006 * tokens) * (aligned ? 1.0 : 1.23) + 0.0104 * (p.m < tokens ? p.m : tokens);
+            offer(tokens, 0, 3.2 + larger(rounds * tile, weights / 4.6));
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -577,7 +598,7 @@ int32_t rb_linear_i8(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* x_scales,
     RB_TRY(kernel_status_word(ctx, &p.status));
     const uint32_t pairs = resident_pairs(ctx);
     if (pairs == 0) return fail(RB_STATUS, "%s: configuring the kernel failed", what);
-    const Plan plan = plan_of(p, (uint32_t)ctx->sm_count, pairs);
+    const Plan plan = plan_of(p, (uint32_t)k, (uint32_t)ctx->sm_count, pairs);
     if (y->dtype == RB_F32) return launch<float>(ctx, p, pw, px, (uint32_t)k, plan, pairs);
     if (y->dtype == RB_BF16) return launch<bf>(ctx, p, pw, px, (uint32_t)k, plan, pairs);
     return launch<__half>(ctx, p, pw, px, (uint32_t)k, plan, pairs);

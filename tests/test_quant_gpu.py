@@ -188,6 +188,14 @@ def test_linear_types(client, m, n, k, dtype, bias):
     linear_case(client, m, n, k, dtype, bias)
 
 
+@pytest.mark.parametrize("m,n,k", [(3, 65, 16), (4, 65, 4112), (5, 65, 16), (5, 4705, 1168), (5, 67, 880), (5, 67, 944), (18, 9473, 16), (17, 5183, 1744), (17, 2201, 960),
+                                   (18, 995, 912), (33, 9603, 16), (35, 5155, 3232), (35, 2867, 1824), (33, 1671, 1456), (390, 11055, 16), (65, 9523, 16), (68, 6307, 4928),
+                                   (68, 3129, 2880), (70, 1867, 2800), (194, 9797, 16), (600, 5003, 2064)])
+def test_linear_of_every_tile_and_split(client, m, n, k):
+    """Sizes at which each tile width with each split of K is the quickest, with ragged edges in all three directions."""
+    linear_case(client, m, n, k, BF16, bias=True)
+
+
 @pytest.mark.parametrize("m", [1, 20, 600])
 def test_linear_largest_sums(client, m):
     """-128 times -128 over the largest K is the largest sum that 32 bits hold."""
