@@ -500,9 +500,6 @@ __global__ void __launch_bounds__(256, 8) dequant_kernel(const int8_t* q, const 
     constexpr int PER = 16 / sizeof(T), UNROLL = 32 / PER;         // 32 elements a thread
     typedef Pack<int8_t, PER> Bytes;
     const Index vectors = (Index)(total / PER), base = (Index)blockIdx.x * 256 * UNROLL + threadIdx.x;
-    Index rows[UNROLL];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) rows[u] = divide((base + u * 256) * PER, by_width);
     Bytes b[UNROLL];
     float scale[UNROLL];
     rb::predecessor_done();
@@ -511,16 +508,16 @@ __global__ void __launch_bounds__(256, 8) dequant_kernel(const int8_t* q, const 
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) b[u] = streamed(reinterpret_cast<const Bytes*>(q) + base + u * 256);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) scale[u] = scales[rows[u]];
+        for (int u = 0; u < UNROLL; ++u) scale[u] = scales[divide((base + u * 256) * PER, by_width)];
     } else {
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) if (base + u * 256 < vectors) { b[u] = streamed(reinterpret_cast<const Bytes*>(q) + base + u * 256); scale[u] = scales[rows[u]]; }
+        for (int u = 0; u < UNROLL; ++u) if (base + u * 256 < vectors) { b[u] = streamed(reinterpret_cast<const Bytes*>(q) + base + u * 256); scale[u] = scales[divide((base + u * 256) * PER, by_width)]; }
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         const Index v = base + u * 256;
         if (v >= vectors) break;
-        const Index row = rows[u];
+        const Index row = divide(v * PER, by_width);
         uint32_t col = (uint32_t)(v * PER - row * (Index)width);
         const float s = scale[u];
         float f[PER], by[PER];
