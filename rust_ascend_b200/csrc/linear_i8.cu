@@ -104,7 +104,7 @@ __device__ __forceinline__ void put(const LinearParams& p, uint32_t token, uint3
 
 // ---------------------------------------------------------------------------------------------------------------------
 // One to four tokens: bound by the bytes of W and, for small layers, by latency.  A warp reads R rows of W, so that a load of x (from
-// L1) serves R times, and has four to eight vectors of 16 bytes a lane in flight: the next round's loads leave before this round's
+// L1) serves R times, and has four to eight vectors of 16 bytes a lane in flight: the next step's loads leave before this step's
 // products.  6144 x 4096, one token: 5.9 us = 4.2 TB/s with the launch; 14336 x 4096: 10.8 us = 5.4 TB/s.
 template <typename Out, int M, int R>
 __global__ void __launch_bounds__(128) linear_i8_row_kernel(const int8_t* x, const int8_t* w, const LinearParams p, const uint32_t k) {
