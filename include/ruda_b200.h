@@ -362,7 +362,8 @@ RB_API int32_t rb_linear_i8(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* x_
  * [rows, top_k], 0 <= top_k <= RB_MAX_TOP and <= V, both NULL when top_k is 0.  A row whose id is ignore_index has log_probs 0;
  * its other outputs are those of its logits.  An id outside [0, V) is never used as an index: its row counts as ignored, and a
  * synchronous context returns RB_INVALID_TENSOR for the call.  Logits of -inf have probability 0;
- * a row without any finite logit (its lse is -inf), or with a NaN or +inf, gives NaN. */
+ * a row without any finite logit (its lse is -inf), or with a NaN or +inf, gives NaN.  The same call gives the same bits; how a row's sums are
+ * ordered, and with it their last bits, follows from the number of rows, V and the rows' alignment. */
 RB_API int32_t rb_token_log_probs(rb_ctx* ctx, const rb_tensor* logits, const rb_tensor* ids, float scale, int64_t ignore_index,
                                   const rb_tensor* log_probs, const rb_tensor* lse, const rb_tensor* entropy, uint32_t top_k,
                                   const rb_tensor* top_values, const rb_tensor* top_ids);
