@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(const uint4* table, cons
 }
 
 // The same lookup for rows that are not a multiple of 16 bytes (width 65 FP32 in examples/embedding_tensor.rs:22): rows move
-// as 4- or 2-byte words.
+// as 4-, 2- or (odd rows of single bytes) 1-byte words.
 template <typename I, typename W>
 __global__ void __launch_bounds__(256) embedding_words_kernel(const W* table, const I* ids, W* out, uint64_t count, uint32_t row_words,
                                                              uint64_t vocab, int* bad) {
@@ -376,14 +376,14 @@ int32_t rb_embedding(rb_ctx* ctx, const rb_tensor* table, const rb_tensor* ids, 
     int* bad = (int*)ctx->workspace;
     RB_CUDA(ctx, "cudaMemsetAsync", cudaMemsetAsync(bad, 0, sizeof(int), ctx->stream));
     if (row_bytes % 16 != 0) {
-        const bool w4 = row_bytes % 4 == 0;
-        const uint32_t words = (uint32_t)(row_bytes / (w4 ? 4 : 2));
-        unsigned gw = grid_for(ctx, count * words);
-        const bool i32 = ids->dtype == RB_I32;
-        if (w4 && i32) embedding_words_kernel<int32_t, uint32_t><<<gw, 256, 0, ctx->stream>>>((const uint32_t*)pt, (const int32_t*)pi, (uint32_t*)po, count, words, table->shape[0], bad);
-        else if (w4) embedding_words_kernel<int64_t, uint32_t><<<gw, 256, 0, ctx->stream>>>((const uint32_t*)pt, (const int64_t*)pi, (uint32_t*)po, count, words, table->shape[0], bad);
-        else if (i32) embedding_words_kernel<int32_t, uint16_t><<<gw, 256, 0, ctx->stream>>>((const uint16_t*)pt, (const int32_t*)pi, (uint16_t*)po, count, words, table->shape[0], bad);
-        else embedding_words_kernel<int64_t, uint16_t><<<gw, 256, 0, ctx->stream>>>((const uint16_t*)pt, (const int64_t*)pi, (uint16_t*)po, count, words, table->shape[0], bad);
+        const uint32_t word = row_bytes % 4 == 0 ? 4 : row_bytes % 2 == 0 ? 2 : 1;
+        const uint32_t words = (uint32_t)(row_bytes / word);
+        const unsigned gw = grid_for(ctx, count * words);
+#define RB_WORDS(W) do { \
+        if (ids->dtype == RB_I32) embedding_words_kernel<int32_t, W><<<gw, 256, 0, ctx->stream>>>((const W*)pt, (const int32_t*)pi, (W*)po, count, words, table->shape[0], bad); \
+        else embedding_words_kernel<int64_t, W><<<gw, 256, 0, ctx->stream>>>((const W*)pt, (const int64_t*)pi, (W*)po, count, words, table->shape[0], bad); } while (0)
+        if (word == 4) RB_WORDS(uint32_t); else if (word == 2) RB_WORDS(uint16_t); else RB_WORDS(uint8_t);
+#undef RB_WORDS
         RB_TRY(after_launch(ctx, "embedding"));
         if (ctx->synchronous) {
             int h = 0; cudaMemcpy(&h, bad, sizeof(int), cudaMemcpyDeviceToHost);
