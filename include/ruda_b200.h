@@ -355,7 +355,7 @@ RB_API int32_t rb_linear_i8(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* x_
 /* ---- scores of single tokens ------------------------------------------------------------------------------------------ */
 #define RB_MAX_TOP 64
 /* This entry has no counterpart in the reference (its loss, src/nn/causal_lm.rs:118-196, keeps only the sum).  With z = scale *
- * logits (scale > 0: one over the temperature) and lse = log(sum(exp(z))), for every row: log_probs = z[id] - lse, lse, entropy =
+ * logits (scale positive and finite: one over the temperature) and lse = log(sum(exp(z))), for every row: log_probs = z[id] - lse, lse, entropy =
  * lse - sum(softmax(z) z), and the top_k largest entries with their log probabilities, ordered by logit (largest first, equal
  * logits by lowest index; a NaN counts as the largest).  logits F32, BF16 or F16 [.., V], row-strided; ids I32 or I64 with one
  * value per row; log_probs, lse and entropy (the last nullable) FP32 with one value per row; top_values FP32 and top_ids I32

@@ -54,6 +54,7 @@ __device__ __forceinline__ float max_nan(float a, float b) { float y; asm("max.N
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr float LEAST = -1000.0f;       // 2^-1000 is 0
+constexpr float SMALLEST_NORMAL = 1.17549435e-38f, LARGEST = 3.402823466e38f;
 
 // Integer that orders values as the top list does: larger value, larger key; both zeros alike; every NaN on top.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -326,9 +327,10 @@ __device__ __noinline__ void exact_candidates(Shared<THREADS>& sh, const T* row,
 
 // A whole row by one block, for the rows that the fast form does not answer: nothing but masks, infinities, NaN, scales far from one.
 // The exponent is (x - M) c with M the largest element itself, held at -1000 and above, where a logit of -inf then counts as 0.
-// m of the result is M, not its product with c.
+// m of the result is M, not its product with c.  Where c = scale log2(e) leaves FP32's normal range the scale and log2(e) are multiplied in
+// one after the other, and a difference that leaves it (two finite logits under a scale below 2^-120) is formed from halves.
 template <typename T, int THREADS>
-__device__ __noinline__ Stats careful_row(Shared<THREADS>& sh, const T* row, uint32_t vocab, float c) {
+__device__ __noinline__ Stats careful_row(Shared<THREADS>& sh, const T* row, uint32_t vocab, float scale, float c) {
     constexpr int WARPS = THREADS / 32;
     float most = -INFINITY;
     for (uint32_t i = threadIdx.x; i < vocab; i += THREADS) most = max_nan(most, to_f32(row[i]));
@@ -338,9 +340,14 @@ __device__ __noinline__ Stats careful_row(Shared<THREADS>& sh, const T* row, uin
     if ((threadIdx.x & 31) == 0) sh.most[threadIdx.x >> 5] = most;
     __syncthreads();
     for (int w = 0; w < WARPS; ++w) most = max_nan(most, sh.most[w]);
+    const bool normal = c >= SMALLEST_NORMAL && c <= LARGEST;
     float s = 0.f, t = 0.f;
     for (uint32_t i = threadIdx.x; i < vocab; i += THREADS) {
-        const float d = fmaxf((to_f32(row[i]) - most) * c, LEAST), e = ex2(d);
+        const float x = to_f32(row[i]), gap = x - most;
+        float d = normal ? gap * c : gap * scale * LOG2E;
+        if (gap < -LARGEST) d = (0.5f * x - 0.5f * most) * scale * (2.f * LOG2E);
+        d = fmaxf(d, LEAST);
+        const float e = ex2(d);
         s += e; t = fmaf(e, d, t);
     }
 #pragma unroll
@@ -485,10 +492,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_scores_kernel(c
             const bool fast = !a.careful && st.m > a.start && fabsf(st.m) < 1048576.0f;      // beyond 2^20 the rounding of m itself would be felt in d
             float reference, logs;               // log p of x is ln2 (c x - reference) - logs, or scale (x - reference) - logs
             if (fast) { reference = st.m; logs = LN2 * log2f(st.s); }
-            else { st = careful_row<T, THREADS>(sh, row, a.vocab, a.c); reference = st.m; logs = logf(st.s); }
+            else { st = careful_row<T, THREADS>(sh, row, a.vocab, a.scale, a.c); reference = st.m; logs = logf(st.s); }
             const float lse = fast ? fmaf(LN2, reference, logs) : fmaf(reference, a.scale, logs);
             auto log_p = [&](float x) {
-                if (!fast) return fmaf(x - reference, a.scale, -logs);
+                if (!fast) {
+                    const float gap = x - reference;
+                    return gap < -LARGEST ? fmaf((0.5f * x - 0.5f * reference) * a.scale, 2.f, -logs) : fmaf(gap, a.scale, -logs);
+                }
                 return x < a.low ? fmaf(x, a.scale, -lse) : fmaf(LN2, fmaf(x, a.c, -reference), -logs);      // c x of a mask's lowest value would overflow
             };
             if (tid == 0) {
@@ -517,10 +527,12 @@ struct GradArgs {
     uint32_t vocab, segments; uint64_t rows;
 };
 
-// -(g + h (log p + H)) p scale, with log p = z - lse held above a value whose exponential is 0 (a NaN stays)
-__device__ __forceinline__ float gradient(float x, float scale, float lse, float g, float h, float hh) {
+// -(g + h (log p + H)) p, and g more at the row's token, with log p = z - lse held above a value whose exponential is 0 (a NaN stays); the
+// scale comes last, so that a product that leaves FP32's range before it meets p does no harm.
+__device__ __forceinline__ float gradient(float x, float scale, float lse, float g, float h, float entropy, bool hot) {
     const float lp = max_nan(fmaf(x, scale, -lse), LEAST);
-    return -ex2(lp * LOG2E) * fmaf(h, lp, g + hh);
+    const float f = -ex2(lp * LOG2E) * fmaf(h, lp + entropy, g);
+    return (hot ? f + g : f) * scale;
 }
 
 template <typename T>
@@ -553,21 +565,25 @@ __global__ void __launch_bounds__(THREADS, 5) token_scores_grad_kernel(const Gra
     T* out = static_cast<T*>(a.out) + r * a.ldo;
     int64_t id = a.wide_ids ? static_cast<const int64_t*>(a.ids)[r] : (int64_t) static_cast<const int32_t*>(a.ids)[r];
     const bool scored = id != a.ignore && id >= 0 && id < (int64_t)a.vocab;
-    const float g = scored ? a.g[r] * a.scale : 0.f, h = a.h ? a.h[r] * a.scale : 0.f, hh = a.h ? h * a.entropy[r] : 0.f;
+    const float g0 = scored ? a.g[r] : 0.f, h0 = a.h ? a.h[r] : 0.f, entropy = a.h ? a.entropy[r] : 0.f;
+    const float g = g0 * a.scale, h = h0 * a.scale, hh = h * entropy;
     // from 2^22 on FP32 steps by half and more: z - lse would not be a log probability
     const float lse = fabsf(a.lse[r]) < 4194304.0f ? a.lse[r] : __int_as_float(0x7fc00000);
     const uint32_t hot = scored ? (uint32_t)id : 0xffffffffu;
-    const bool idle = g == 0.f && h == 0.f;      // an unscored row (whose logits may be anything) or no upstream: zeros
+    const bool idle = g0 == 0.f && h0 == 0.f;      // an unscored row (whose logits may be anything) or no upstream: zeros
     // The vectors' form: d = c x - lse log2(e), two elements an instruction, 2^d (-(g + h H) - h ln2 d).  Logits below `low`, from where
-    // 2^d is 0, are lifted to it, so that d stays finite; where the type cannot hold that value (scales far below one), one by one.
+    // 2^d is 0, are lifted to it, so that d stays finite; where the type cannot hold that value (scales far below one), or c or the bracket
+    // (d is above -1444) would leave FP32, one by one.
     const float c = a.scale * LOG2E, base = -lse * LOG2E, slope = -h * LN2, level = -(g + hh), low = (lse + LEAST) / a.scale;
-    const bool fast = !(low < (std::is_same<T, __half>::value ? -65000.f : -1e38f));       // a NaN row goes either way
+    const bool fast = !(low < (std::is_same<T, __half>::value ? -65000.f : -1e38f)) && !(c > LARGEST) && !(fabsf(level) + 1001.f * fabsf(h) > LARGEST);      // a NaN row goes either way
     // one element, with the arithmetic that it has in a vector: results do not depend on the alignment of the rows
     auto one = [&](uint32_t i, T x) {
         if (idle) return 0.f;
-        float f;
-        if (fast) { alignas(4) const T pair[2] = {x, x}; float xa, xb; lifted<T>(pair, low, xa, xb); const float d = fmaf(xa, c, base); f = fmaf(slope, d, level) * ex2(d); }
-        else f = gradient(to_f32(x), a.scale, lse, g, h, hh);
+        if (!fast) return gradient(to_f32(x), a.scale, lse, g0, h0, entropy, i == hot);
+        alignas(4) const T pair[2] = {x, x};
+        float xa, xb;
+        lifted<T>(pair, low, xa, xb);
+        const float d = fmaf(xa, c, base), f = fmaf(slope, d, level) * ex2(d);
         return i == hot ? f + g : f;
     };
     const RowView<T> view(row, a.vocab);
