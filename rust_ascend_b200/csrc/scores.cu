@@ -341,15 +341,21 @@ __device__ __noinline__ Stats careful_row(Shared<THREADS>& sh, const T* row, uin
     __syncthreads();
     for (int w = 0; w < WARPS; ++w) most = max_nan(most, sh.most[w]);
     const bool normal = c >= SMALLEST_NORMAL && c <= LARGEST;
-    float s = 0.f, t = 0.f;
-    for (uint32_t i = threadIdx.x; i < vocab; i += THREADS) {
+    auto take_one = [&](uint32_t i, float& s, float& t) {
         const float x = to_f32(row[i]), gap = x - most;
         float d = normal ? gap * c : gap * scale * LOG2E;
         if (gap < -LARGEST) d = (0.5f * x - 0.5f * most) * scale * (2.f * LOG2E);
         d = fmaxf(d, LEAST);
         const float e = ex2(d);
         s += e; t = fmaf(e, d, t);
+    };
+    // two sums a thread, as in the fast form: with 128 threads one sum would be V / 128 roundings long
+    float s = 0.f, t = 0.f, s1 = 0.f, t1 = 0.f;
+    for (uint32_t i = threadIdx.x; i < vocab; i += 2 * THREADS) {
+        take_one(i, s, t);
+        if (vocab - i > THREADS) take_one(i + THREADS, s1, t1);
     }
+    s += s1; t += t1;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, d); t += __shfl_xor_sync(0xffffffffu, t, d); }
     __syncthreads();
