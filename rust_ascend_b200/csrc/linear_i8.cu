@@ -16,6 +16,7 @@
 //     under the products of the next.  Bound: the tensor cores.
 #include "common.cuh"
 
+#include "linear_plan.h"
 #include "schedule.h"
 #include "sm100.cuh"
 
@@ -24,8 +25,8 @@ namespace {
 using namespace sm100;
 using bf = __nv_bfloat16;
 
-constexpr int ROWS = 128;        // weight rows per CTA (TMEM lanes)
-constexpr int BK = 128;          // K per stage: one 128-byte swizzle row
+constexpr int ROWS = RB_LINEAR_ROWS;        // weight rows per CTA (TMEM lanes)
+constexpr int BK = RB_LINEAR_BK;            // K per stage: one 128-byte swizzle row
 constexpr int UMMA_K = 32;       // 32 bytes
 constexpr int A_BYTES = ROWS * BK;
 constexpr int THREADS = 192;     // producer, issuer, four epilogue warps
@@ -33,7 +34,7 @@ constexpr int THREADS = 192;     // producer, issuer, four epilogue warps
 struct LinearParams {
     uint32_t m, n, num_kb;
     uint32_t tiles_t, tiles_n;       // token tiles, weight tiles
-    uint32_t tokens;                 // pair kernel: tokens of a whole tile, a multiple of 32 within 256
+    uint32_t tokens;                 // pair kernel: tokens of a whole tile, 128 or 256
     uint32_t split, items;           // pair kernel: whole tiles, all work items (see rb_gemm_plan)
     const float* sx; const float* sw; const float* bias;
     void* y;
@@ -485,7 +486,7 @@ template <typename Out>
 int32_t launch_pair(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, uint32_t k, uint32_t pairs, uint32_t tokens) {
     p.tokens = tokens;
     p.tiles_n = (p.n + 2 * ROWS - 1) / (2 * ROWS); p.tiles_t = (p.m + tokens - 1) / tokens;
-    rb_gemm_plan(p.tiles_n * p.tiles_t, pairs, tokens % 64 == 0, p.split, p.items);
+    rb_gemm_plan(p.tiles_n * p.tiles_t, pairs, true, p.split, p.items);
     if (p.items < pairs) pairs = p.items;
     CUtensorMap mw, mx, mxh;
     if (!byte_map(&mw, w, p.n, k, ROWS) || !byte_map(&mx, x, p.m, k, tokens / 2) || !byte_map(&mxh, x, p.m, k, tokens / 4))
@@ -495,25 +496,19 @@ int32_t launch_pair(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, 
 }
 
 template <typename Out>
-int32_t launch_rows(rb_ctx* ctx, const LinearParams& p, const void* w, const void* x, uint32_t k) {
+int32_t launch_rows(rb_ctx* ctx, const LinearParams& p, const void* w, const void* x, uint32_t k, uint32_t rows) {
     const int8_t* xp = static_cast<const int8_t*>(x); const int8_t* wp = static_cast<const int8_t*>(w);
-    // More rows a warp (R) mean fewer loads of x and fewer warps.  us for n x k and m tokens at R = 1 / 2 / 4: 1024 x 4096, 1: 3.0 / 3.7 / 5.3;
-    // 6144 x 4096, 1: 6.8 / 5.9 / 7.2; 6144 x 4096, 4: - / 9.1 / 6.9; 4096 x 4096, 4: 6.6 / 6.2 / 6.1.
-    const uint32_t sms = (uint32_t)ctx->sm_count;
 #define RB_ROWS(M, R) rb::launch_behind(ctx, linear_i8_row_kernel<Out, M, R>, (p.n + 4 * R - 1) / (4 * R), 128, 0, 0, true, xp, wp, p, k)
-    if (p.m == 1) { if (p.n <= 32 * sms) RB_ROWS(1, 1); else RB_ROWS(1, 2); }
-    else if (p.m == 2) { if (p.n <= 16 * sms) RB_ROWS(2, 1); else RB_ROWS(2, 2); }
-    else { if (p.n <= 32 * sms) RB_ROWS(4, 2); else RB_ROWS(4, 4); }
+    if (p.m == 1) { if (rows == 1) RB_ROWS(1, 1); else RB_ROWS(1, 2); }
+    else if (p.m == 2) { if (rows == 1) RB_ROWS(2, 1); else RB_ROWS(2, 2); }
+    else { if (rows == 2) RB_ROWS(4, 2); else RB_ROWS(4, 4); }
 #undef RB_ROWS
     return rb::after_launch(ctx, "8-bit linear (rows)");
 }
 
-// tokens: width of a tile; parts: CTAs that share K.  parts 0: CTA pairs; tokens 0: rows.
-struct Plan { uint32_t tokens, parts; };
-
 template <typename Out>
-int32_t launch(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, uint32_t k, const Plan& plan, uint32_t pairs) {
-    if (plan.tokens == 0) return launch_rows<Out>(ctx, p, w, x, k);
+int32_t launch(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, uint32_t k, const rb_linear_plan& plan, uint32_t pairs) {
+    if (plan.tokens == 0) return launch_rows<Out>(ctx, p, w, x, k, plan.rows);
     if (plan.parts == 0) return launch_pair<Out>(ctx, p, w, x, k, pairs, plan.tokens);
     switch (plan.tokens) {
         case 16: return launch_few<Out, 16>(ctx, p, w, x, k, plan.parts);
@@ -521,48 +516,6 @@ int32_t launch(rb_ctx* ctx, LinearParams& p, const void* w, const void* x, uint3
         case 64: return launch_few<Out, 64>(ctx, p, w, x, k, plan.parts);
         default: return launch_few<Out, 128>(ctx, p, w, x, k, plan.parts);
     }
-}
-
-// Which kernel, by the sizes alone: the least of estimated times in us.  The constants were fitted to 4774 sizes of 3 to 700 tokens (random ones
-// and layers of 1024 to 28672 outputs), each timed with every tile and split; what is chosen takes 1.02 to 1.03 of the best one's time
-// on average, 1.12 in nine of ten cases, where borders in tokens and K took 1.22 and 1.11 on average.  The terms are the kernels' own:
-//   * few tokens: a start; the stages of a CTA's part of K, each at its latency or, where two CTAs share an SM, at the rate of the SM's
-//     port to L2 (rows that do not start on cache lines pass it slower), at least the weights' way out of DRAM; the stores; the join
-//     of the parts; a further wave, which clusters reach earlier because they do not fill every SM.
-//   * pairs: a start and the rounds of tiles.
-Plan plan_of(const LinearParams& p, uint32_t k, uint32_t sms, uint32_t pairs) {
-    // One or two tokens, and up to four over short rows: no tensor core, no set-up (one token, 6144 x 4096: 5.9 us against 7.8; four tokens: K of
-    // 1536 0.85 to 1.09 of the tiles' time, K of 4096 1.1 to 1.2).
-    if (p.m <= 2 || (p.m <= 4 && p.num_kb < 24)) return {0, 0};
-    auto up = [](uint64_t a, uint64_t b) { return (a + b - 1) / b; };
-    auto larger = [](double a, double b) { return a > b ? a : b; };
-    const bool aligned = k % BK == 0;
-    const double weights = (double)p.n * k * 1e-6;
-    Plan best{256, 0};
-    double least = 1e300;
-    auto offer = [&](uint32_t tokens, uint32_t parts, double us) { if (us < least) { least = us; best = {tokens, parts}; } };
-    for (uint32_t tokens = 16; tokens <= 128 && (tokens == 16 || tokens < 2 * p.m); tokens *= 2) {
-        const double used = p.m < tokens ? p.m : tokens;
-        const double latency = 0.195 + 0.0009 * tokens, port = 0.0009 * (ROWS + tokens) * (aligned ? 1.0 : 1.37);
-        for (uint32_t parts = 1; parts <= 8 && parts <= p.num_kb; parts *= 2) {
-            const uint64_t ctas = up(p.n, ROWS) * up(p.m, tokens) * parts;
-            const uint32_t spare = sms > 32 ? sms : 33;
-            const uint32_t seats = parts < 4 ? sms : parts == 4 ? spare - 8 : spare * 13 / 16, wave = parts < 4 ? 2 * sms : parts == 4 ? 2 * spare - 32 : seats;
-            const uint64_t share = up(ctas, seats);      // CTAs of the fullest SM
-            const double body = up(p.num_kb, parts) * ((double)(share / 2) * larger(latency, 2 * port) + (double)(share % 2) * larger(latency, port)) + 0.0125 * used * share / parts;
-            offer(tokens, parts, 1.85 + 1.4 * (double)(up(ctas, wave) - 1) + larger(body, weights / 5.1) + (parts > 1 ? 0.78 + 0.031 * used : 0.0));
-        }
-    }
-    if (p.m > 16) {
-        for (uint32_t tokens = 128; tokens <= 256; tokens *= 2) {
-            const uint64_t tiles = up(p.n, 2 * ROWS) * up(p.m, tokens), rest = tiles % pairs;
-            const double halves = tiles < pairs ? 0.72 : 0.63;      // a short last round runs as half tiles, partly under the round in front
-            const double rounds = (double)(tiles / pairs) + (rest == 0 ? 0.0 : 2 * rest <= pairs ? halves : 1.0);
-            const double tile = p.num_kb * (0.150 + 0.0006 * tokens) * (aligned ? 1.0 : 1.23) + 0.0104 * (p.m < tokens ? p.m : tokens);
-            offer(tokens, 0, 3.2 + larger(rounds * tile, weights / 4.6));
-        }
-    }
-    return best;
 }
 
 }  // namespace
@@ -598,7 +551,7 @@ int32_t rb_linear_i8(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* x_scales,
     RB_TRY(kernel_status_word(ctx, &p.status));
     const uint32_t pairs = resident_pairs(ctx);
     if (pairs == 0) return fail(RB_STATUS, "%s: configuring the kernel failed", what);
-    const Plan plan = plan_of(p, (uint32_t)k, (uint32_t)ctx->sm_count, pairs);
+    const rb_linear_plan plan = rb_linear_plan_of(p.m, p.n, (uint32_t)k, (uint32_t)ctx->sm_count, pairs);
     if (y->dtype == RB_F32) return launch<float>(ctx, p, pw, px, (uint32_t)k, plan, pairs);
     if (y->dtype == RB_BF16) return launch<bf>(ctx, p, pw, px, (uint32_t)k, plan, pairs);
     return launch<__half>(ctx, p, pw, px, (uint32_t)k, plan, pairs);
