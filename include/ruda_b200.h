@@ -140,8 +140,10 @@ RB_API int32_t rb_host_free(rb_ctx* ctx, void* host);
  * stream.  rb_profile_end synchronises and returns the elapsed device milliseconds. */
 RB_API int32_t rb_profile_begin(rb_ctx* ctx);
 RB_API int32_t rb_profile_end(rb_ctx* ctx, float* milliseconds);
-/* Caps the number of SMs the persistent GEMM occupies (0 = all), leaving the rest to a collective that runs beside
- * it.  No counterpart in the reference, whose collectives and kernels never overlap (runtime/hccl.rs:290-305). */
+/* Caps the number of SMs that the tensor-core kernels occupy (GEMMs, attention, rb_linear_i8; 0 = all; pairs of SMs keep at least one
+ * pair), leaving the rest to a collective that runs beside them: a CTA of theirs takes an SM's shared memory whole.  Row-wise kernels, maps
+ * and the token scores are not capped.
+ * No counterpart in the reference, whose collectives and kernels never overlap (runtime/hccl.rs:290-305). */
 RB_API int32_t rb_set_sm_limit(rb_ctx* ctx, int32_t sm_limit);
 /* Records everything enqueued on the context between begin and end (kernels, copies, collectives with their
  * cross-stream fences) into a CUDA graph, and replays it with one launch.  The reference launches and synchronises

@@ -42,7 +42,7 @@ struct rb_ctx {
     bool poisoned = false;             // set after a failed launch or synchronisation
     rb_stats stats{};
     int sm_count = 0;
-    int sm_limit = 0;                  // 0: persistent kernels use every SM
+    int sm_limit = 0;                  // 0: the tensor-core kernels use every SM
     std::unordered_map<uint64_t, cudaGraphExec_t> graphs;
     uint64_t next_graph = 1;
     bool capturing = false;

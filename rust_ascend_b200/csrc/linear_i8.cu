@@ -478,7 +478,7 @@ uint32_t resident_pairs(rb_ctx* ctx) {
     });
     if (e != cudaSuccess) return 0;
     uint32_t pairs = (uint32_t)once.value[ctx->device];
-    if (ctx->sm_limit > 0 && (uint32_t)ctx->sm_limit / 2 < pairs) pairs = (uint32_t)ctx->sm_limit < 2 ? 1 : (uint32_t)ctx->sm_limit / 2;
+    if (ctx->sm_limit > 0 && (uint32_t)ctx->sm_limit / 2 < pairs) pairs = (uint32_t)ctx->sm_limit < 2 ? 1 : (uint32_t)ctx->sm_limit / 2;      // at least one pair
     return pairs;
 }
 
@@ -551,7 +551,8 @@ int32_t rb_linear_i8(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* x_scales,
     RB_TRY(kernel_status_word(ctx, &p.status));
     const uint32_t pairs = resident_pairs(ctx);
     if (pairs == 0) return fail(RB_STATUS, "%s: configuring the kernel failed", what);
-    const rb_linear_plan plan = rb_linear_plan_of(p.m, p.n, (uint32_t)k, (uint32_t)ctx->sm_count, pairs);
+    const bool limited = ctx->sm_limit > 0 && ctx->sm_limit < ctx->sm_count;
+    const rb_linear_plan plan = rb_linear_plan_of(p.m, p.n, (uint32_t)k, (uint32_t)(limited ? ctx->sm_limit : ctx->sm_count), pairs, limited);
     if (y->dtype == RB_F32) return launch<float>(ctx, p, pw, px, (uint32_t)k, plan, pairs);
     if (y->dtype == RB_BF16) return launch<bf>(ctx, p, pw, px, (uint32_t)k, plan, pairs);
     return launch<__half>(ctx, p, pw, px, (uint32_t)k, plan, pairs);

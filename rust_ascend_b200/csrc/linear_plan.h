@@ -25,12 +25,16 @@ inline uint32_t rb_linear_rows_of(uint32_t m, uint32_t n, uint32_t sms) {
 //     port to L2 (rows that do not start on cache lines pass it slower), at least the weights' way out of DRAM; the stores; the join
 //     of the parts; a further wave, which clusters reach earlier because they do not fill every SM.
 //   * pairs: a start and the rounds of tiles.
-// sms, pairs: SMs and CTA pairs that there are.
-inline rb_linear_plan rb_linear_plan_of(uint32_t m, uint32_t n, uint32_t k, uint32_t sms, uint32_t pairs) {
+// sms, pairs: SMs and CTA pairs that the call may use.  limited: other SMs are to stay free.  The pairs keep to their number by themselves; the
+// other kernels are offered only while they have no more CTAs than that, so that they cannot spread further.
+inline rb_linear_plan rb_linear_plan_of(uint32_t m, uint32_t n, uint32_t k, uint32_t sms, uint32_t pairs, bool limited) {
     const uint32_t num_kb = (k + RB_LINEAR_BK - 1) / RB_LINEAR_BK;
     // One or two tokens, and up to four over short rows: no tensor core, no set-up (one token, 6144 x 4096: 5.9 us against 7.8; four tokens: K of
     // 1536 0.85 to 1.09 of the tiles' time, K of 4096 1.1 to 1.2).
-    if (m <= 2 || (m <= 4 && num_kb < 24)) return {0, 0, rb_linear_rows_of(m, n, sms)};
+    if (m <= 2 || (m <= 4 && num_kb < 24)) {
+        const uint32_t rows = rb_linear_rows_of(m, n, sms);
+        if (!limited || (n + 4 * rows - 1) / (4 * rows) <= sms) return {0, 0, rows};
+    }
     auto up = [](uint64_t a, uint64_t b) { return (a + b - 1) / b; };
     auto larger = [](double a, double b) { return a > b ? a : b; };
     const bool aligned = k % RB_LINEAR_BK == 0;
@@ -43,6 +47,7 @@ inline rb_linear_plan rb_linear_plan_of(uint32_t m, uint32_t n, uint32_t k, uint
         const double latency = 0.195 + 0.0009 * tokens, port = 0.0009 * (RB_LINEAR_ROWS + tokens) * (aligned ? 1.0 : 1.37);
         for (uint32_t parts = 1; parts <= 8 && parts <= num_kb; parts *= 2) {
             const uint64_t ctas = up(n, RB_LINEAR_ROWS) * up(m, tokens) * parts;
+            if (limited && ctas > sms) break;
             const uint32_t spare = sms > 32 ? sms : 33;
             const uint32_t seats = parts < 4 ? sms : parts == 4 ? spare - 8 : spare * 13 / 16, wave = parts < 4 ? 2 * sms : parts == 4 ? 2 * spare - 32 : seats;
             const uint64_t share = up(ctas, seats);      // CTAs of the fullest SM
@@ -50,7 +55,7 @@ inline rb_linear_plan rb_linear_plan_of(uint32_t m, uint32_t n, uint32_t k, uint
             offer(tokens, parts, 1.85 + 1.4 * (double)(up(ctas, wave) - 1) + larger(body, weights / 5.1) + (parts > 1 ? 0.78 + 0.031 * used : 0.0));
         }
     }
-    if (m > 16) {
+    if (m > 16 || limited) {
         for (uint32_t tokens = 128; tokens <= 256; tokens *= 2) {
             const uint64_t tiles = up(n, 2 * RB_LINEAR_ROWS) * up(m, tokens), rest = tiles % pairs;
             const double halves = tiles < pairs ? 0.72 : 0.63;      // a short last round runs as half tiles, partly under the round in front
