@@ -138,24 +138,28 @@ struct QuantArgs {
     float eps;
 };
 
-// SiLU(x) u = x u / (1 + 2^(-x log2 e)): one exponential and one reciprocal.  From x = -87.3 on down the reciprocal's argument leaves
-// the normal range and the result is -0; an infinite or NaN x gives NaN or infinity, which marks the row.
+// SiLU(x) u = x u / (1 + 2^(-x log2 e)): one exponential and one reciprocal.  The reciprocal flushes results below 2^-126 (from x = -87.3 on
+// down, which large u make visible), so it is taken of a quarter of the denominator and its product with a quarter may be denormal (4096 x 14336
+// BF16: 56.2 us, 53.9 without; products left four times as large and undone with the row's factor: 55.7).  From x = -88.8 on down the
+// exponential is infinite and the result -0; an infinite or NaN x gives NaN or infinity, which marks the row.
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float rcp(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 template <int VEC>
 __device__ __forceinline__ void silu_mul(float (&x)[VEC], const float (&u)[VEC]) {
-    constexpr float LOG2E = 1.44269504088896340736f;
+    constexpr float LOG2E = 1.44269504088896340736f, QUARTER = 0.25f;
     if constexpr (VEC % 2 != 0) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) x[j] = __fmul_rn(__fmul_rn(x[j], rcp(1.0f + ex2(x[j] * -LOG2E))), u[j]);
+        for (int j = 0; j < VEC; ++j) x[j] = __fmul_rn(__fmul_rn(x[j], __fmul_rn(rcp(__fmaf_rn(ex2(x[j] * -LOG2E), QUARTER, QUARTER)), QUARTER)), u[j]);
     } else {
 #pragma unroll
         for (int j = 0; j < VEC; j += 2) {
             float e = x[j], f = x[j + 1];
             mul2(e, f, -LOG2E, -LOG2E);
-            e = ex2(e); f = ex2(f);
-            add2(e, f, 1.0f, 1.0f);
-            mul2(x[j], x[j + 1], rcp(e), rcp(f));
+            float d = QUARTER, g = QUARTER;
+            fma2(d, g, ex2(e), ex2(f), QUARTER, QUARTER);
+            d = rcp(d); g = rcp(g);
+            mul2(d, g, QUARTER, QUARTER);
+            mul2(x[j], x[j + 1], d, g);
             mul2(x[j], x[j + 1], u[j], u[j + 1]);
         }
     }
