@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(THREADS, 5) token_scores_grad_kernel(const Gra
     int64_t id = a.wide_ids ? static_cast<const int64_t*>(a.ids)[r] : (int64_t) static_cast<const int32_t*>(a.ids)[r];
     const bool scored = id != a.ignore && id >= 0 && id < (int64_t)a.vocab;
     const float g0 = scored ? a.g[r] : 0.f, h0 = a.h ? a.h[r] : 0.f, entropy = a.h ? a.entropy[r] : 0.f;
-    const float g = g0 * a.scale, h = h0 * a.scale, hh = h * entropy;
+    const float g = __fmul_rn(g0, a.scale), h = __fmul_rn(h0, a.scale), hh = __fmul_rn(h, entropy);
     // from 2^22 on FP32 steps by half and more: z - lse would not be a log probability
     const float lse = fabsf(a.lse[r]) < 4194304.0f ? a.lse[r] : __int_as_float(0x7fc00000);
     const uint32_t hot = scored ? (uint32_t)id : 0xffffffffu;
