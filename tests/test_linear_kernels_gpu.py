@@ -13,6 +13,16 @@ from test_quant_gpu import linear_case
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def limit(client):
+    """Sets the context's SM limit.  Every test here begins and ends without one, whatever was set before."""
+    def set_to(sms):
+        _check(client._lib.rb_set_sm_limit(client._ctx, C.c_int32(sms)))
+    set_to(0)
+    yield set_to
+    set_to(0)
+
+
 @pytest.mark.parametrize("size", SIZES, ids=str)
 @pytest.mark.parametrize("dtype", [DType.F32, DType.BF16, DType.F16])
 def test_linear(client, size, dtype):
@@ -31,14 +41,6 @@ def kernel_of(client, m, n, k):
     (name, blocks), = launched(client, call)
     assert "linear_i8" in name
     return next(kind for kind in ("row", "few", "pair") if f"linear_i8_{kind}_kernel" in name), blocks
-
-
-@pytest.fixture
-def limit(client):
-    def set_to(sms):
-        _check(client._lib.rb_set_sm_limit(client._ctx, C.c_int32(sms)))
-    yield set_to
-    set_to(0)
 
 
 @pytest.mark.parametrize("size", SIZES, ids=str)
