@@ -327,15 +327,18 @@ RB_API int32_t rb_gemm_no_alloc(rb_ctx* ctx, const rb_tensor* a, const rb_tensor
 
 /* ---- rows held in 8 bits, and the linear on them ------------------------------------------------------------------- */
 /* Rules shared by the entries of this section.  A row of values y is held as signed 8-bit integers q and one FP32 scale:
- * scale = max(max|y| / 127, 2^-126), q = y / scale rounded to the nearest integer (ties to even), so |q| <= 127 and
- * |q * scale - y| <= scale / 2.  A row that holds a NaN or an infinity gets a NaN scale and zeros, so that everything computed from
+ * scale = max(max|y| / 127, 2^-126), q = y / scale rounded to the nearest integer, so |q| <= 127.  The quotient is formed as a product with
+ * 127 / max|y|, so q is within 1/2 + 2^-15 of y / scale, and a value that close to the middle between two integers may go to either (exact
+ * ties go to the even one where 127 / max|y| is exact); for SiLU * up the approximate exponential and reciprocal come on top, some units in the last place
+ * of y.  The scale itself is rounded to FP32.  A row that holds a NaN or an infinity gets a NaN scale and zeros, so that everything computed from
  * it is NaN.  Row-strided inputs: the last axis is contiguous and the leading axes step through rows at one distance (a column
  * range of a wider tensor); only the element's own alignment is required of them. */
 /* This entry has no counterpart in the reference.  rb_rms_norm (delta NULL, x_out NULL) or rb_add_rms_norm (both given: the sum
  * is rounded to x's type and stored to x_out, which may be x itself) whose result leaves in 8 bits: y = s * rsqrt(mean(s^2) +
  * epsilon) * w is quantised by rows into q (I8, x's shape) and scales (FP32, one value per row).  x F32, BF16 or F16, any width;
  * weight in x's type or F32.  One pass over x: the normalised row is never stored.  The products s * w are formed in FP32 before the
- * root is divided out: a row in which one leaves FP32's range counts as one that holds an infinity. */
+ * root is divided out: a row in which one leaves FP32's range counts as one that holds an infinity.  A sum of squares beyond FP32 gives zeros,
+ * as in rb_rms_norm. */
 RB_API int32_t rb_rms_norm_quant(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* delta, const rb_tensor* weight, double epsilon,
                                  const rb_tensor* x_out, const rb_tensor* q, const rb_tensor* scales);
 /* This entry has no counterpart in the reference.  Quantises rows: y = x, or, with `up` given, y = SiLU(x) * up in FP32 (the
@@ -350,7 +353,7 @@ RB_API int32_t rb_dequantize_rows(rb_ctx* ctx, const rb_tensor* q, const rb_tens
  * integers: y[m, n] = (sum over k of x[m, k] w[n, k]) * (x_scales[m] * w_scales[n]) (+ bias[n]).  x I8 [.., K], w I8 [N, K], x_scales
  * FP32 with one value per row of x, w_scales FP32 [N], bias FP32 [N] or NULL, y F32, BF16 or F16 [.., N].  The integer sum is exact
  * (32-bit), so the result does not depend on how the work is split; it is rounded to FP32 once, scaled, biased and rounded to
- * y's type.  Any number of rows, any N; K a multiple of 16 within 131056 (the largest whose sum cannot leave 32 bits). */
+ * y's type; the product of the two scales is formed in FP32 first.  Any number of rows, any N; K a multiple of 16 within 131056 (the largest whose sum cannot leave 32 bits). */
 RB_API int32_t rb_linear_i8(rb_ctx* ctx, const rb_tensor* x, const rb_tensor* x_scales, const rb_tensor* w, const rb_tensor* w_scales,
                             const rb_tensor* bias, const rb_tensor* y);
 
@@ -372,7 +375,8 @@ RB_API int32_t rb_token_log_probs(rb_ctx* ctx, const rb_tensor* logits, const rb
 /* This entry has no counterpart in the reference.  Gradient of rb_token_log_probs with respect to the logits, from the saved lse
  * and entropy: dlogits[v] = scale * (g (onehot(id)[v] - p[v]) - h p[v] (log p[v] + entropy)), p = exp(z - lse), g = grad_log_probs of
  * the row (0 for ignored rows), h = grad_entropy (NULL: 0; entropy may then be NULL too).  A row with g = h = 0 gets zeros whatever
- * its logits hold.  p inherits the rounding of lse (|lse| 2^-24, relative); an lse of 2^22 or more in magnitude (a row of nothing but
+ * its logits hold.  p is off by up to 4 (|z| + |lse|) 2^-24, relative (the roundings of z and lse in units of log 2, and of lse itself), and counts as 0
+ * below 2^-126; an lse of 2^22 or more in magnitude (a row of nothing but
  * a mask's lowest value) no longer tells the logits apart and gives a NaN row.  dlogits has the type and shape of the logits, may be row-strided, and may be the logits tensor itself; columns
  * between its rows keep their bits. */
 RB_API int32_t rb_token_log_probs_backward(rb_ctx* ctx, const rb_tensor* logits, const rb_tensor* ids, float scale, int64_t ignore_index,

@@ -9,7 +9,8 @@
 // so no N needs alignment.
 //
 // Three kernels:
-//   * one to four tokens: a warp per weight row (or several), 16-byte loads and dot products of four bytes; no set-up but the launch.
+//   * one or two tokens, and up to four over short rows: a warp per weight row (or several), 16-byte loads and dot products of four bytes; no
+//     set-up but the launch.
 //   * few tokens: one tile of 128 weight rows x TOKENS tokens per cluster, K split over the cluster's CTAs so that all SMs stream
 //     weights; the parts are added through distributed shared memory.  Bound: the bytes of W.
 //   * many tokens: CTA pairs (cta_group::2) on 256 x 256 tiles, persistent, two accumulators in TMEM so that the store of one tile runs
@@ -106,7 +107,7 @@ __device__ __forceinline__ void put(const LinearParams& p, uint32_t token, uint3
 // ---------------------------------------------------------------------------------------------------------------------
 // One to four tokens: bound by the bytes of W and, for small layers, by latency.  A warp reads R rows of W, so that a load of x (from
 // L1) serves R times, and has four to eight vectors of 16 bytes a lane in flight: the next step's loads leave before this step's
-// products.  6144 x 4096, one token: 5.9 us = 4.2 TB/s with the launch; 14336 x 4096: 10.8 us = 5.4 TB/s.
+// products.  6144 x 4096, one token, recorded: 5.9 us = 4.2 TB/s with the launch; 14336 x 4096: 10.8 us = 5.4 TB/s.
 template <typename Out, int M, int R>
 __global__ void __launch_bounds__(128) linear_i8_row_kernel(const int8_t* x, const int8_t* w, const LinearParams p, const uint32_t k) {
     constexpr int UNROLL = 4 / R;
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(128) linear_i8_row_kernel(const int8_t* x, con
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Few tokens.  Stages are sized so that two CTAs share an SM (one streams while the other starts or stores).  17 x 4096 x 14336: 13.4 us =
+// Few tokens.  Stages are sized so that two CTAs share an SM (one streams while the other starts or stores).  17 x 4096 x 14336, recorded: 13.2 us =
 // 4.4 TB/s of weights; about 4 us of any call are the launch, the first load's latency and the join of the parts.
 template <int TOKENS> struct Few {
     static constexpr int B_BYTES = TOKENS * BK;
@@ -309,7 +310,7 @@ linear_i8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 // Many tokens: pairs of CTAs on tiles of 256 weight rows x 256 tokens.  Each CTA keeps 128 of the weight rows in its TMEM and loads
 // its weight rows and half of the tokens; rank 0 issues the products and every completion reaches the barriers of both.
 // Every CTA fetches its own tiles.  A last round that would use at most half of the pairs runs as tiles of 128 tokens.
-// 4096 x 14336 x 4096: tensor pipe 94 % busy, 143 us = 3.4 POP/s from a cool start, 170 us = 2.8 in a loop under the power cap.
+// 4096 x 14336 x 4096: tensor pipe busy in 88 % of all cycles, 143 us = 3.4 POP/s from a cool start, 170 us = 2.8 in a loop under the power cap.
 // Rows that do not start on cache lines (K not a multiple of 128) cost about 1.4 times as much: each 128-byte row of a copy then
 // takes two lines through the SM's port to L2 (1003 x 5001: 22 us at K = 4096, 30 at 4112).
 constexpr int PAIR_TOKENS = 256;

@@ -651,8 +651,9 @@ void launch_scores(rb_ctx* ctx, const ScoreArgs& a) {
     const int resident = counted == cudaSuccess && once.value[ctx->device] > 0 ? once.value[ctx->device] : 1;
     const uint64_t slots = (uint64_t)ctx->sm_count * resident, bytes = (uint64_t)a.vocab * sizeof(T);
     // A row is one block's work where the rows fill the GPU or are short; few long rows are split over clusters.  us at 1 / 2 / 4 / 8 blocks
-    // a row: 4 x 128000 BF16 with 20 alternatives 14.6 / 11.9 / 8.9 / 9.5, without 5.0 / 4.3 at 4 / 8; 4 x 32000 BF16 with 20 6.2 / 7.8 (the join
-    // of the lists costs what the split saves).
+    // a row, BF16: 4 x 128000 with 20 alternatives 11.8 / 10.3 / 8.9 / 9.1, without 8.4 / 6.4 / 4.8 / 4.0; 4 x 32000 with 20 6.3 / 7.2 / 8.1 / 9.4
+    // (the join of the lists costs what the split saves).  With alternatives the curves cross late and flat, later for more rows: 20 at 100 KB 8.3 / 8.3 / 8.0 for 4
+    // rows, 9.4 / 11.3 / 10.8 for 64; at 160 KB 9.2 / 9.4 / 9.0 and 11.6 / 13.5 / 14.1; at 200 KB 11.2 / 10.3 / 9.1 and 14.4 / 15.9 / 14.4.
     uint32_t log_parts = 0;
     if (bytes >= (TOP ? 160u : 96u) * 1024)
         while (log_parts < (TOP ? 2 : 3) && a.rows << (log_parts + 1) <= 3ull * ctx->sm_count) ++log_parts;
