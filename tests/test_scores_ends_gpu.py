@@ -68,3 +68,26 @@ def test_gradient_at_the_ends(client, dtype, scale, out):
     off = np.abs(got.astype(np.float64) - want) - (gradient_error(xv, ids, scale, g, h, dtype) * (1 + half) + (half + 6 * U) * np.abs(want) + smallest)
     assert off.max() <= 0, (off.max(), np.isnan(got).any())
     assert not got[1, 100:].any()
+
+
+@pytest.mark.parametrize("dtype,scale", [(F16, 1e-30), (F16, 1e-3), (F16, 0.014), (F16, 0.02), (BF16, 1e-35), (BF16, 1e-37), (F32, 1e-34), (F32, 1e-36)])
+@pytest.mark.parametrize("with_entropy", [False, True])
+@pytest.mark.parametrize("upstream", [1.0, 1e30])
+def test_gradient_on_both_sides_of_the_scale_that_goes_element_by_element(client, dtype, scale, with_entropy, upstream):
+    """Nearly uniform rows under scales at which the masks' stand-in no longer fits the type, and just above; gradients of order one, or large ones of the scores."""
+    scale = float(np.float32(scale))
+    rng = np.random.default_rng([int(-np.log10(scale)), int(dtype)])
+    rows, vocab = 5, 1003
+    x, xv = R.hold(np.clip(rng.standard_normal((rows, vocab)) * min(3 / scale, 60000 if dtype == F16 else 1e38) / 4, -65504 if dtype == F16 else -3e38, 65504 if dtype == F16 else 3e38), dtype)
+    ids = rng.integers(0, vocab, rows)
+    ids[3] = -100
+    size = min(upstream, 0.1 / scale)
+    g, h = (size * rng.standard_normal(rows)).astype(np.float32), (size * 0.3 * rng.standard_normal(rows)).astype(np.float32) * with_entropy
+    t, s = call(client, x, xv, ids, dtype, scale, 0)
+    up = client.upload
+    d = RT.token_log_probs_backward(client, t, up(ids), s[1], s[2] if with_entropy else None, up(g), up(h) if with_entropy else None, scale=scale)
+    got, want = R.read(client, d).astype(np.float64), R.scores_gradient(xv, ids, scale, -100, g, h)
+    half = R.half_step(dtype)
+    smallest = {F32: 2.0 ** -149, BF16: 2.0 ** -133, F16: 2.0 ** -24}[dtype]
+    off = np.abs(got - want) - (gradient_error(xv, ids, scale, g, h, dtype) * (1 + half) + (half + 6 * U) * np.abs(want) + smallest)
+    assert off.max() <= 0, off.max()
